@@ -242,6 +242,70 @@ int32_t yule_cuda_multihead_attention_static(yule_cuda_ctx *ctx, yule_buffer q, 
 int32_t yule_cuda_embed_gather(yule_cuda_ctx *ctx, yule_buffer table, uint32_t gguf_type,
                                uint32_t dim, uint32_t token, yule_buffer out);
 
+/* ── a batch of sequences served together (no counterpart in the reference, which serves one sequence per ModelRunner,
+ *    yule-infer/src/lib.rs:169-216) ──────────────────────────────────────────
+ * Lengths, adapters and drafts are read on the device, so a captured call can be replayed with others.  The calls share a scratch
+ * that the context grows on demand; growing is not possible while a graph is being captured, so run one call of the
+ * same sizes before yule_cuda_graph_begin. */
+
+/* Decode attention of n_seqs sequences that share a prefix, n_query query tokens each (1, or 1 + drafted tokens).  Keys of every row: positions
+ * [0, prefix_len) of the prefix caches, then the sequence's own positions.  q and out: [n_seqs][n_query] tokens of n_heads * head_dim floats, q_stride /
+ * out_stride floats apart.  prefix_k / prefix_v: [prefix_len] positions prefix_stride floats apart; tail_k / tail_v: [n_seqs][tail_capacity] positions
+ * tail_stride apart.  tail_lens: n_seqs words, the positions that sequence b's own caches hold, its query tokens' among them (the newest n_query; more than
+ * tail_capacity counts as tail_capacity): query token t sees its own and earlier ones, tail_lens[b] - (n_query - 1 - t) positions, none if that is negative.
+ * A row that sees nothing is zero.  Scores, soft-max and head grouping as yule_cuda_multihead_attention.  Handles of a prefix_len
+ * or tail_capacity of 0 are not looked at.  A value that is not finite in a position that a row sees makes that row's output not finite; what no
+ * row of a sequence sees is not read.  head_dim a multiple of 4, at most 256; strides multiples of 4; n_query at most 64. */
+typedef struct yule_prefix_attention {
+    uint32_t head_dim, n_heads, n_kv_heads;
+    uint32_t prefix_len, n_seqs, n_query, tail_capacity;
+    uint32_t q_stride, out_stride, prefix_stride, tail_stride;
+} yule_prefix_attention;
+int32_t yule_cuda_prefix_attention(yule_cuda_ctx *ctx, yule_buffer q, yule_buffer prefix_k, yule_buffer prefix_v,
+                                   yule_buffer tail_k, yule_buffer tail_v, yule_buffer tail_lens, yule_buffer out,
+                                   const yule_prefix_attention *shape);
+
+/* Low-rank adapters of many requests beside a shared projection (whose result, of quantized_matmul_batched say, is `base`):
+ *     output[i] = base[i] + scales[a] * up[a] * (down[a] * input[i]),   a = row_adapter[i],
+ * and output[i] = base[i] for a row whose row_adapter is n_adapters or more.  base and output may be the same buffer; rows without an adapter are then left
+ * alone.  down: [n_adapters][max_rank][n_cols], up: [n_adapters][n_rows][max_rank], both F16 or F32 (gguf_type); ranks: n_adapters words, the
+ * rank of each adapter (more than max_rank counts as max_rank; rows and columns beyond it are not used); scales: n_adapters floats; row_adapter: batch words; input
+ * [batch][x_stride], base and output [batch][out_stride] floats.  Rows of one adapter need not be neighbours, but are cheaper so.  n_cols and x_stride
+ * multiples of 4; max_rank at most 256. */
+typedef struct yule_adapters {
+    uint32_t gguf_type, n_adapters, max_rank, n_rows, n_cols;
+    uint32_t batch, x_stride, out_stride;
+} yule_adapters;
+int32_t yule_cuda_adapter_matmul_batched(yule_cuda_ctx *ctx, yule_buffer down, yule_buffer up, yule_buffer ranks,
+                                         yule_buffer scales, yule_buffer row_adapter, yule_buffer input, yule_buffer base,
+                                         yule_buffer output, const yule_adapters *shape);
+
+/* Verification of drafted tokens: how many of a sequence's drafts stand, and the token after them, distributed as the target model alone would give it.
+ * target_logits: [n_seqs][n_draft + 1] rows of vocab_size floats, target_stride apart (row t: after t drafts); draft_logits: [n_seqs][n_draft] rows
+ * draft_stride apart, or handle 0 for drafts that were not drawn from a distribution (looked up, say); drafts: [n_seqs][n_draft] words; draft_lens: n_seqs
+ * words, how many of them there are (handle 0: n_draft each; more count as n_draft); random: [n_seqs][n_draft + 1] floats in [0, 1).  With p, q the soft-max of
+ * logits / temperature, draft t is accepted while random[t] * q(draft) < p(draft) (q = 1 without draft logits); at the first that is not, the token is
+ * drawn from max(0, p - q), after the last accepted one from p: in index order, the first whose running sum exceeds random[n_draft] times the
+ * whole.  Sums and exponentials are in 64 bits.  greedy != 0: drafts are accepted while they are the target's largest logit (ties to the highest
+ * index, sampler.rs:150-163), the token is that logit's; draft_logits, random and temperature are then not looked at.
+ * out_tokens: [n_seqs][n_draft + 1] words, the accepted drafts, the token after them, then 0xFFFFFFFF; out_accepted: n_seqs words, the number of accepted
+ * drafts.  A logit that is NaN or -infinity is a token that cannot be; a row of those accepts nothing and gives 0xFFFFFFFF; a draft outside the
+ * vocabulary is not accepted.  Penalties and cut-offs of yule_cuda_sample are not applied. */
+typedef struct yule_verification {
+    uint32_t vocab_size, n_seqs, n_draft;
+    uint32_t target_stride, draft_stride;
+    float temperature;
+    uint32_t greedy;
+} yule_verification;
+int32_t yule_cuda_verify_drafts(yule_cuda_ctx *ctx, yule_buffer target_logits, yule_buffer draft_logits, yule_buffer drafts,
+                                yule_buffer draft_lens, yule_buffer random, yule_buffer out_tokens,
+                                yule_buffer out_accepted, const yule_verification *shape);
+
+/* Device address of a buffer, for hosts that look at it with another library on the same GPU instead of copying it.  It lies there until it is freed; what others do
+ * with it is not in the order of this context's stream (synchronize before and after), and weights written through it do not drop the copy
+ * that yule_cuda_prepare_weights made. */
+int32_t yule_cuda_buffer_address(yule_cuda_ctx *ctx, yule_buffer handle, uint64_t *out_address);
+
 /* Record a sequence of this context's compute/copy_buffer calls once and replay it: between
  * graph_begin and graph_end the calls are captured into a CUDA graph instead of executed (the
  * blocking entry points — copy_from_device, synchronize, free, destroy — must not be called

@@ -1,0 +1,295 @@
+"""Verification of drafted tokens (csrc/verify.cu) against its definition in 64 bits.  Tokens are whole numbers: they have to be equal.  The random numbers are drawn so that none lies
+within 2^-36 of a border (in units of the whole), far more than sums in 64 bits are off by."""
+
+import numpy as np
+import pytest
+
+from yule_b200 import CudaB200Backend, YuleGpuError
+
+pytestmark = pytest.mark.gpu
+NONE = 0xFFFFFFFF
+
+
+def soft(row, temperature):
+    """Probabilities of a row of logits, or None where no token can be."""
+    x = np.asarray(row, np.float64).copy()
+    x[np.isnan(x)] = -np.inf
+    x = np.minimum(x, np.finfo(np.float32).max)
+    if x.max() == -np.inf:
+        return None
+    e = np.exp((x - x.max()) / np.float64(np.float32(temperature)))
+    return e / e.sum()
+
+
+def reference(c):
+    tokens, accepted, close = np.full((c.B, c.K + 1), NONE, np.uint32), np.zeros(c.B, np.uint32), 1.0
+    for b in range(c.B):
+        k = c.K if c.lens is None else min(int(c.lens[b]), c.K)
+        a = 0
+        q = None
+        while a < k:
+            x, p = int(c.drafts[b, a]), soft(c.target[b, a], c.temperature)
+            q = None
+            if c.greedy:
+                row = np.where(np.isnan(c.target[b, a]), -np.inf, np.minimum(c.target[b, a], np.finfo(np.float32).max))
+                fits = p is not None and x < c.V and x == c.V - 1 - int(row[::-1].argmax())
+            else:
+                q = np.zeros(c.V)
+                if c.draft is None:
+                    if x < c.V:
+                        q[x] = 1.0
+                else:
+                    d = soft(c.draft[b, a], c.temperature)
+                    q = q if d is None else d
+                fits = x < c.V and p is not None and float(c.random[b, a]) * q[x] < p[x]
+                if x < c.V and p is not None:
+                    close = min(close, abs(float(c.random[b, a]) * q[x] - p[x]) / max(p[x], 1e-300))
+            if not fits:
+                break
+            a += 1
+        accepted[b] = a
+        tokens[b, :a] = c.drafts[b, :a]
+        p = soft(c.target[b, a], c.temperature)
+        if p is None:
+            continue
+        if c.greedy:
+            row = np.where(np.isnan(c.target[b, a]), -np.inf, np.minimum(c.target[b, a], np.finfo(np.float32).max))
+            tokens[b, a] = c.V - 1 - int(row[::-1].argmax())
+            continue
+        w = np.maximum(p - q, 0) if a < k else p
+        run = np.cumsum(w)
+        if run[-1] > 0:
+            goal = float(c.random[b, c.K]) * run[-1]
+            over = np.nonzero((run > goal) & (w > 0))[0]
+            tokens[b, a] = over[0] if len(over) else np.nonzero(w > 0)[0][-1]
+            close = min(close, np.abs(run[w > 0] - goal).min() / run[-1])
+    return tokens, accepted, close
+
+
+class Call:
+    def __init__(self, B=4, K=3, V=500, temperature=0.8, by="model", lens=None, greedy=False, seed=0, near=0.6, spread=2.0, pad=0):
+        r = np.random.default_rng(seed)
+        self.B, self.K, self.V, self.temperature, self.greedy, self.pad = B, K, V, temperature, greedy, pad
+        self.target = (r.standard_normal((B, K + 1, V)) * spread).astype(np.float32)
+        self.draft = (self.target[:, :K] + near * r.standard_normal((B, K, V))).astype(np.float32) if by == "model" else None
+        like = self.draft if by == "model" else self.target[:, :K] + 0.3 * r.standard_normal((B, K, V))
+        self.drafts = (like / temperature + (r.gumbel(size=(B, K, V)) if by == "model" else 0)).argmax(-1).astype(np.uint32)
+        self.lens = None if lens is None else np.asarray(lens, np.uint32)
+        self.random = r.random((B, K + 1)).astype(np.float32)
+        self.random[self.random >= 1] = 0.5
+
+    def upload(self, b):
+        def wide(a):
+            return np.concatenate([a.reshape(-1, self.V), np.full((a.shape[0] * a.shape[1], self.pad), np.inf, np.float32)], 1)
+
+        self.h = dict(target=b.upload(wide(self.target)), draft=b.upload(wide(self.draft)) if self.draft is not None else None, drafts=b.upload(self.drafts),
+                      lens=b.upload(self.lens) if self.lens is not None else None, random=b.upload(self.random), tokens=b.upload(np.full(self.B * (self.K + 1) + 8, 5, np.uint32)),
+                      accepted=b.upload(np.full(self.B + 8, 5, np.uint32)))
+        return self
+
+    def run(self, b):
+        h = self.h
+        b.verify_drafts(h["target"], h["draft"], h["drafts"], h["lens"], h["random"], h["tokens"], h["accepted"], self.V, self.B, self.K, temperature=self.temperature,
+                        greedy=self.greedy, target_stride=self.V + self.pad, draft_stride=self.V + self.pad)
+
+    def got(self, b):
+        n = self.B * (self.K + 1)
+        t, a = b.download(self.h["tokens"], n + 8, np.uint32), b.download(self.h["accepted"], self.B + 8, np.uint32)
+        assert (t[n:] == 5).all() and (a[self.B:] == 5).all()
+        return t[:n].reshape(self.B, -1), a[:self.B]
+
+    def check(self, b):
+        tokens, accepted, close = reference(self)
+        assert close > 2.0 ** -36, "a random number on a border says nothing"
+        got = self.got(b)
+        assert (got[1] == accepted).all() and (got[0] == tokens).all()
+        return accepted
+
+    def free(self, b):
+        for h in self.h.values():
+            if h:
+                b.free(h)
+
+
+def go(b, **kw):
+    c = Call(**kw).upload(b)
+    c.run(b)
+    accepted = c.check(b)
+    c.free(b)
+    return accepted
+
+
+WAYS = pytest.mark.parametrize("way", [dict(by="model"), dict(by="lookup"), dict(by="lookup", greedy=True)], ids=["model", "lookup", "greedy"])
+
+
+@WAYS
+@pytest.mark.parametrize("V", [1, 2, 31, 255, 256, 1000, 1024, 1025, 4095, 4096, 4097, 8192, 8193, 32000, 50257, 128256])
+def test_vocabularies(backend, way, V):
+    go(backend, V=V, seed=V, B=3 if V > 10000 else 6, **way)
+
+
+@WAYS
+def test_all_numbers_of_accepted_drafts_come_up(backend, way):
+    seen = np.concatenate([go(backend, B=32, K=3, V=300, seed=s, near=0.5, **way) for s in range(4)])
+    assert set(seen.tolist()) == {0, 1, 2, 3}
+
+
+@WAYS
+@pytest.mark.parametrize("K", [1, 2, 7, 31, 32, 33, 70, 256])
+def test_numbers_of_drafts(backend, way, K):
+    """Drafts that nearly always stand, so that runs are long."""
+    go(backend, B=3, K=K, V=40, near=0.01, seed=K, spread=3.0, **way)
+
+
+@WAYS
+def test_lengths_of_the_drafts(backend, way):
+    go(backend, B=7, K=4, V=200, lens=[0, 1, 2, 3, 4, 5, NONE], near=0.05, **way)
+
+
+@WAYS
+@pytest.mark.parametrize("pad", [1, 3, 8])
+def test_strides(backend, way, pad):
+    go(backend, pad=pad, V=1001, **way)
+
+
+@pytest.mark.parametrize("temperature", [1e-6, 0.05, 0.5, 1.0, 3.0, 100.0, 1e6])
+def test_temperatures(backend, temperature):
+    go(backend, temperature=temperature, B=8, V=300)
+    go(backend, temperature=temperature, B=8, V=300, by="lookup")
+
+
+@WAYS
+def test_logits_of_any_size(backend, way):
+    for spread in (1e-30, 1e-3, 50.0, 1e4, 1e30):
+        go(backend, spread=spread, B=6, V=300, near=0.0 if spread > 1e5 else 0.3 * spread, **way)
+
+
+@WAYS
+def test_tokens_that_cannot_be(backend, way):
+    """NaN and −infinity are tokens without probability, rows of them have none at all; +infinity is the largest number."""
+    c = Call(B=8, K=3, V=300, **way)
+    c.target[0, :, ::2] = -np.inf
+    c.target[1, :, 5:] = np.nan
+    c.target[2] = -np.inf
+    c.target[3, 1] = np.nan
+    c.target[4, 0, 7], c.target[4, 0, 9] = np.inf, np.inf
+    c.target[5, 3, :] = -np.finfo(np.float32).max
+    if c.draft is not None:
+        c.draft[6, 0] = -np.inf
+        c.draft[7, 0, c.drafts[7, 0]] = -np.inf
+    c.upload(backend).run(backend)
+    c.check(backend)
+
+
+@WAYS
+def test_drafts_outside_the_vocabulary(backend, way):
+    c = Call(B=4, K=3, V=300, near=0.01, **way)
+    c.drafts[0, 0], c.drafts[1, 1], c.drafts[2, 2] = 300, NONE, 1 << 31
+    c.upload(backend).run(backend)
+    c.check(backend)
+
+
+def test_equal_distributions_accept_everything(backend):
+    c = Call(B=16, K=3, V=500, near=0.0)
+    c.upload(backend).run(backend)
+    assert (c.check(backend) == 3).all()
+
+
+def test_random_numbers_at_the_ends(backend):
+    for u in (0.0, np.nextafter(np.float32(1), np.float32(0))):
+        c = Call(B=8, K=3, V=300)
+        c.random[:] = u
+        c.upload(backend).run(backend)
+        tokens, accepted, _ = reference(c)
+        got = c.got(backend)
+        assert (got[0] == tokens).all() and (got[1] == accepted).all()
+    # what is no random number gives a token of the vocabulary all the same
+    for u in (1.0, 2.0, -1.0, np.nan, np.inf):
+        c = Call(B=8, K=3, V=300)
+        c.random[:] = u
+        c.upload(backend).run(backend)
+        tokens, accepted = c.got(backend)
+        for b in range(8):
+            assert accepted[b] <= 3 and tokens[b, accepted[b]] < 300 and (tokens[b, accepted[b] + 1:] == NONE).all()
+
+
+def test_greedy_ties_go_to_the_highest_index(backend):
+    c = Call(B=2, K=2, V=9000, by="lookup", greedy=True)
+    c.target[:] = 0
+    c.target[:, :, [3, 4000, 8500]] = 2.0
+    c.drafts[0], c.drafts[1] = [8500, 8500], [8500, 4000]
+    c.upload(backend).run(backend)
+    tokens, accepted = c.got(backend)
+    assert accepted.tolist() == [2, 1] and tokens.tolist() == [[8500, 8500, 8500], [8500, 8500, NONE]]
+
+
+def test_tokens_are_distributed_as_the_target(backend):
+    """Many sequences of one distribution: the first token's frequencies are the target's, within five standard deviations, although the drafts' are others."""
+    B, V = 20000, 6
+    c = Call(B=B, K=1, V=V, temperature=1.0)
+    p, q = np.array([.3, .05, .2, .25, .1, .1]), np.array([.1, .3, .3, .1, .15, .05])
+    r = np.random.default_rng(1)
+    c.target[:] = np.log(p)
+    c.draft[:] = np.log(q)
+    c.drafts[:, 0] = r.choice(V, B, p=q)
+    c.random = r.random((B, 2)).astype(np.float32)
+    c.upload(backend).run(backend)
+    tokens, _ = c.got(backend)
+    share = np.bincount(tokens[:, 0], minlength=V) / B
+    assert (np.abs(share - p) < 5 * np.sqrt(p * (1 - p) / B)).all()
+
+
+def test_captured_and_replayed_with_other_inputs(backend):
+    c = Call(B=5, K=3, V=3000, lens=[3, 3, 3, 3, 3]).upload(backend)
+    c.run(backend)
+    backend.graph_begin()
+    c.run(backend)
+    g = backend.graph_end()
+    for seed in (5, 6):
+        d = Call(B=5, K=3, V=3000, lens=[0, 1, 2, 3, 3], seed=seed)
+        for name in ("target", "draft", "drafts", "lens", "random"):
+            setattr(c, name, getattr(d, name))
+            backend.copy_to_device(getattr(d, name), c.h[name])
+        backend.graph_launch(g)
+        c.check(backend)
+    backend.graph_destroy(g)
+
+
+def test_refusals(backend):
+    c = Call(lens=[1, 2, 3, 3]).upload(backend)
+    h = c.h
+    good = [h["target"], h["draft"], h["drafts"], h["lens"], h["random"], h["tokens"], h["accepted"], 500, 4, 3]
+    small = backend.allocate(4)
+
+    def refused(code, at, value, **more):
+        args = list(good)
+        args[at] = value
+        with pytest.raises(YuleGpuError) as e:
+            backend.verify_drafts(*args, **more)
+        assert e.value.code == code
+
+    for at in range(7):
+        refused(3, at, small)
+    for at in range(5):
+        refused(1, at, h["tokens"])
+        refused(1, at, h["accepted"])
+    refused(1, 5, h["accepted"])
+    refused(2, 4, None)
+    refused(1, 7, 0)
+    refused(3, 7, 501)
+    refused(1, 9, 0)
+    refused(1, 9, 3, temperature=0.0)
+    c.run(backend)
+    c.check(backend)
+
+
+def test_a_capture_cannot_grow_the_scratch():
+    b = CudaB200Backend(0)
+    c = Call().upload(b)
+    b.graph_begin()
+    with pytest.raises(YuleGpuError, match="outside the capture"):
+        c.run(b)
+    b.graph_destroy(b.graph_end())
+    c.run(b)
+    c.check(b)
+    b.close()

@@ -31,6 +31,23 @@ class SamplingParams(C.Structure):
     _fields_ = [("temperature", f32), ("top_p", f32), ("top_k", u32), ("repetition_penalty", f32), ("min_p", f32)]
 
 
+class PrefixAttention(C.Structure):
+    """``yule_prefix_attention`` of include/yule_cuda.h."""
+    _fields_ = [(n, u32) for n in ("head_dim", "n_heads", "n_kv_heads", "prefix_len", "n_seqs", "n_query", "tail_capacity", "q_stride", "out_stride",
+                                   "prefix_stride", "tail_stride")]
+
+
+class Adapters(C.Structure):
+    """``yule_adapters`` of include/yule_cuda.h."""
+    _fields_ = [(n, u32) for n in ("gguf_type", "n_adapters", "max_rank", "n_rows", "n_cols", "batch", "x_stride", "out_stride")]
+
+
+class Verification(C.Structure):
+    """``yule_verification`` of include/yule_cuda.h."""
+    _fields_ = [("vocab_size", u32), ("n_seqs", u32), ("n_draft", u32), ("target_stride", u32), ("draft_stride", u32),
+                ("temperature", f32), ("greedy", u32)]
+
+
 class GgufTensorInfo(C.Structure):
     """``yule_gguf_tensor_info`` of include/yule_cuda.h."""
     _fields_ = [("name", C.c_char_p), ("n_dims", u32), ("shape", u64 * 8), ("gguf_type", u32), ("offset", u64),
@@ -69,6 +86,10 @@ _SIGNATURES = {
     "yule_cuda_multihead_attention": [vp, u64, u64, u64, u64, u32, u32, u32, u32, u32],
     "yule_cuda_multihead_attention_static": [vp, u64, u64, u64, u64, u32, u32, u32, u32, u32],
     "yule_cuda_embed_gather": [vp, u64, u32, u32, u32, u64],
+    "yule_cuda_prefix_attention": [vp, u64, u64, u64, u64, u64, u64, u64, C.POINTER(PrefixAttention)],
+    "yule_cuda_adapter_matmul_batched": [vp, u64, u64, u64, u64, u64, u64, u64, u64, C.POINTER(Adapters)],
+    "yule_cuda_verify_drafts": [vp, u64, u64, u64, u64, u64, u64, u64, C.POINTER(Verification)],
+    "yule_cuda_buffer_address": [vp, u64, C.POINTER(u64)],
     "yule_cuda_graph_begin": [vp],
     "yule_cuda_graph_end": [vp, C.POINTER(u32)],
     "yule_cuda_graph_launch": [vp, u32],

@@ -10,6 +10,7 @@
 
 #include <cstdlib>
 
+#include "batch_args.h"
 #include "internal.h"
 
 namespace yule {
@@ -90,6 +91,35 @@ int32_t ensure_sampler_scratch(yule_cuda_ctx *ctx, size_t n_floats) {
         return fail(YULE_ERR_OUT_OF_MEMORY, "cuda allocation of %zu bytes of sampler scratch failed", n_floats * sizeof(float));
     }
     ctx->sampler_scratch_floats = n_floats;
+    return YULE_OK;
+}
+
+// The scratch of the operators for a batch.  The context's enqueue lock is held.
+static int32_t ensure_batch_scratch(yule_cuda_ctx *ctx, size_t bytes) {
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    if (ctx->batch_scratch_bytes >= bytes) return YULE_OK;
+    if (ctx->capturing)
+        return fail(YULE_ERR_INVALID_ARGUMENT, "the scratch of this call (%zu bytes) cannot grow during graph capture: run the call once outside the capture first", bytes);
+    struct Allowed {  // (as for the GEMM's scratch)
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        Allowed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+        ~Allowed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    } allowed;
+    void *block = nullptr;
+    size_t got = bytes < 2 * ctx->batch_scratch_bytes ? 2 * ctx->batch_scratch_bytes : bytes;
+    cudaError_t e = cudaMalloc(&block, got);
+    if (e == cudaErrorMemoryAllocation && got > bytes) {
+        cudaGetLastError();
+        e = cudaMalloc(&block, got = bytes);
+    }
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        if (e != cudaErrorMemoryAllocation) return fail_cuda(e, "cudaMalloc of the batch scratch");
+        return fail(YULE_ERR_OUT_OF_MEMORY, "cuda allocation of %zu bytes of scratch failed", bytes);
+    }
+    if (ctx->batch_scratch) ctx->retired_scratch.push_back(ctx->batch_scratch);  // launches before this one, and graphs captured earlier, may still use it
+    ctx->batch_scratch = block;
+    ctx->batch_scratch_bytes = got;
     return YULE_OK;
 }
 
@@ -233,6 +263,7 @@ int32_t yule_cuda_destroy(yule_cuda_ctx *ctx) {
     if (ctx->gemm_scratch) cudaFree(ctx->gemm_scratch);
     for (void *p : ctx->retired_scratch) cudaFree(p);
     if (ctx->sampler_scratch) cudaFree(ctx->sampler_scratch);
+    if (ctx->batch_scratch) cudaFree(ctx->batch_scratch);
     cudaStreamDestroy(ctx->stream);
     delete ctx;
     return YULE_OK;
@@ -975,6 +1006,139 @@ int32_t yule_cuda_sample(yule_cuda_ctx *ctx, yule_buffer logits, uint32_t n, con
     // (the word is one for all callers: read before the next one samples)
     YULE_CUDA_TRY(cudaMemcpyAsync(out_token, a.out_token, 4, cudaMemcpyDeviceToHost, ctx->stream));
     YULE_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
+    return YULE_OK;
+}
+
+// ── a batch of sequences served together ───────────────────────────────────────────────────
+
+int32_t yule_cuda_buffer_address(yule_cuda_ctx *ctx, yule_buffer handle, uint64_t *out_address) {
+    CTX_GUARD(ctx);
+    if (!out_address) return fail(YULE_ERR_INVALID_ARGUMENT, "null out_address");
+    FIND(ctx, handle, b);
+    *out_address = (uint64_t)(uintptr_t)b.ptr;
+    return YULE_OK;
+}
+
+int32_t yule_cuda_prefix_attention(yule_cuda_ctx *ctx, yule_buffer q, yule_buffer prefix_k, yule_buffer prefix_v, yule_buffer tail_k, yule_buffer tail_v,
+                                   yule_buffer tail_lens, yule_buffer out, const yule_prefix_attention *shape) {
+    CTX_ENQUEUE(ctx);
+    PrefixNeeds need;
+    if (int32_t rc = check_prefix_attention(shape, &need)) return rc;
+    if (out == q || out == prefix_k || out == prefix_v || out == tail_k || out == tail_v || out == tail_lens)
+        return fail(YULE_ERR_INVALID_ARGUMENT, "the output of prefix_attention cannot be one of its inputs");
+    FIND(ctx, q, Q);
+    FIND(ctx, out, O);
+    NEED_BYTES(Q, need.q, "prefix_attention q");
+    NEED_BYTES(O, need.out, "prefix_attention out");
+    PrefixAttention a;
+    if (shape->prefix_len) {
+        FIND(ctx, prefix_k, K);
+        FIND(ctx, prefix_v, V);
+        NEED_BYTES(K, need.prefix, "prefix_attention prefix_k");
+        NEED_BYTES(V, need.prefix, "prefix_attention prefix_v");
+        a.prefix_k = (const float *)K.ptr, a.prefix_v = (const float *)V.ptr;
+    }
+    if (shape->tail_capacity) {
+        FIND(ctx, tail_k, K);
+        FIND(ctx, tail_v, V);
+        FIND(ctx, tail_lens, L);
+        NEED_BYTES(K, need.tail, "prefix_attention tail_k");
+        NEED_BYTES(V, need.tail, "prefix_attention tail_v");
+        NEED_BYTES(L, need.lens, "prefix_attention tail_lens");
+        a.tail_k = (const float *)K.ptr, a.tail_v = (const float *)V.ptr, a.tail_lens = (const uint32_t *)L.ptr;
+    }
+    a.q = (const float *)Q.ptr, a.out = (float *)O.ptr;
+    a.hd = shape->head_dim, a.n_heads = shape->n_heads, a.n_kv_heads = shape->n_kv_heads;
+    a.prefix_len = shape->prefix_len, a.n_seqs = shape->n_seqs, a.n_query = shape->n_query, a.tail_capacity = shape->tail_capacity;
+    a.q_stride = shape->q_stride, a.out_stride = shape->out_stride, a.prefix_stride = shape->prefix_stride, a.tail_stride = shape->tail_stride;
+    if (int32_t rc = ensure_batch_scratch(ctx, prefix_attention_scratch_bytes(a, ctx->prop.multiProcessorCount))) return rc;
+    a.scratch = ctx->batch_scratch;
+    a.pdl = chain_goes_on(ctx, _chain.armed, _chain.n);
+    LAUNCHED(ctx, launch_prefix_attention(a, ctx->prop.multiProcessorCount, ctx->stream, &_n));
+    chain_output(ctx, O.ptr, need.out);
+    ctx->pdl_chain = true;
+    return YULE_OK;
+}
+
+int32_t yule_cuda_adapter_matmul_batched(yule_cuda_ctx *ctx, yule_buffer down, yule_buffer up, yule_buffer ranks, yule_buffer scales, yule_buffer row_adapter,
+                                         yule_buffer input, yule_buffer base, yule_buffer output, const yule_adapters *shape) {
+    CTX_ENQUEUE(ctx);
+    AdapterNeeds need;
+    if (int32_t rc = check_adapters(shape, &need)) return rc;
+    if (output == down || output == up || output == ranks || output == scales || output == row_adapter || output == input)
+        return fail(YULE_ERR_INVALID_ARGUMENT, "the output of adapter_matmul_batched can be its base, but no other input");
+    FIND(ctx, down, D);
+    FIND(ctx, up, U);
+    FIND(ctx, ranks, R);
+    FIND(ctx, scales, S);
+    FIND(ctx, row_adapter, I);
+    FIND(ctx, input, X);
+    FIND(ctx, base, B);
+    FIND(ctx, output, O);
+    NEED_BYTES(D, need.down, "adapter down");
+    NEED_BYTES(U, need.up, "adapter up");
+    NEED_BYTES(R, need.of_adapters, "adapter ranks");
+    NEED_BYTES(S, need.of_adapters, "adapter scales");
+    NEED_BYTES(I, need.of_rows, "adapter of each row");
+    NEED_BYTES(X, need.input, "adapter input");
+    NEED_BYTES(B, need.output, "adapter base");
+    NEED_BYTES(O, need.output, "adapter output");
+    AdapterBatch a;
+    a.down = D.ptr, a.up = U.ptr, a.ranks = (const uint32_t *)R.ptr, a.row_adapter = (const uint32_t *)I.ptr, a.scales = (const float *)S.ptr, a.x = (const float *)X.ptr;
+    a.base = (const float *)B.ptr, a.out = (float *)O.ptr;
+    a.type = shape->gguf_type, a.n_adapters = shape->n_adapters, a.max_rank = shape->max_rank, a.n_rows = shape->n_rows, a.n_cols = shape->n_cols, a.batch = shape->batch;
+    a.x_stride = shape->x_stride, a.out_stride = shape->out_stride;
+    if (int32_t rc = ensure_batch_scratch(ctx, adapter_scratch_bytes(a, ctx->prop.multiProcessorCount))) return rc;
+    a.scratch = ctx->batch_scratch;
+    a.pdl = chain_goes_on(ctx, _chain.armed, _chain.n);
+    LAUNCHED(ctx, launch_adapters(a, ctx->prop.multiProcessorCount, ctx->stream, &_n));
+    chain_output(ctx, O.ptr, need.output);
+    ctx->pdl_chain = true;
+    return YULE_OK;
+}
+
+int32_t yule_cuda_verify_drafts(yule_cuda_ctx *ctx, yule_buffer target_logits, yule_buffer draft_logits, yule_buffer drafts, yule_buffer draft_lens, yule_buffer random,
+                                yule_buffer out_tokens, yule_buffer out_accepted, const yule_verification *shape) {
+    CTX_ENQUEUE(ctx);
+    VerifyNeeds need;
+    if (int32_t rc = check_verification(shape, draft_logits != 0, &need)) return rc;
+    for (yule_buffer in : {target_logits, draft_logits, drafts, draft_lens, random})
+        if (in && (in == out_tokens || in == out_accepted)) return fail(YULE_ERR_INVALID_ARGUMENT, "an output of verify_drafts cannot be one of its inputs");
+    if (out_tokens == out_accepted) return fail(YULE_ERR_INVALID_ARGUMENT, "verify_drafts has two outputs, in a buffer each");
+    FIND(ctx, target_logits, T);
+    FIND(ctx, drafts, D);
+    FIND(ctx, out_tokens, O);
+    FIND(ctx, out_accepted, A);
+    NEED_BYTES(T, need.target, "verify_drafts target logits");
+    NEED_BYTES(D, need.drafts, "verify_drafts drafts");
+    NEED_BYTES(O, need.places, "verify_drafts tokens");
+    NEED_BYTES(A, need.of_seqs, "verify_drafts accepted");
+    VerifyDrafts a;
+    if (draft_logits && !shape->greedy) {
+        FIND(ctx, draft_logits, Q);
+        NEED_BYTES(Q, need.draft, "verify_drafts draft logits");
+        a.draft = (const float *)Q.ptr;
+    }
+    if (draft_lens) {
+        FIND(ctx, draft_lens, L);
+        NEED_BYTES(L, need.of_seqs, "verify_drafts draft lengths");
+        a.lens = (const uint32_t *)L.ptr;
+    }
+    if (!shape->greedy) {
+        FIND(ctx, random, R);
+        NEED_BYTES(R, need.places, "verify_drafts random numbers");
+        a.random = (const float *)R.ptr;
+    }
+    a.target = (const float *)T.ptr, a.drafts = (const uint32_t *)D.ptr, a.tokens = (uint32_t *)O.ptr, a.accepted = (uint32_t *)A.ptr;
+    a.vocab = shape->vocab_size, a.n_seqs = shape->n_seqs, a.n_draft = shape->n_draft, a.target_stride = shape->target_stride, a.draft_stride = shape->draft_stride;
+    a.temperature = shape->greedy ? 1.f : shape->temperature, a.greedy = shape->greedy != 0;
+    if (int32_t rc = ensure_batch_scratch(ctx, verify_scratch_bytes(a))) return rc;
+    a.scratch = ctx->batch_scratch;
+    a.pdl = chain_goes_on(ctx, _chain.armed, _chain.n);
+    LAUNCHED(ctx, launch_verify_drafts(a, ctx->stream, &_n));
+    chain_output(ctx, O.ptr, need.places);
+    chain_output(ctx, A.ptr, need.of_seqs);
+    ctx->pdl_chain = true;
     return YULE_OK;
 }
 

@@ -94,6 +94,10 @@ struct yule_cuda_ctx {
     // scratch of the device sampler (sampler.cu): probabilities and occurrence counts, plus one word for the pick
     float *sampler_scratch = nullptr;
     size_t sampler_scratch_floats = 0;
+    // scratch of the operators for a batch served together (prefix_attention.cu, adapters.cu, verify.cu), grown on demand: each call's first kernel waits for
+    // all before it, so they can share it
+    void *batch_scratch = nullptr;
+    size_t batch_scratch_bytes = 0;
     // Scratch blocks that were outgrown.  A CUDA graph captured earlier (the runner's steps, a caller's batch)
     // may still replay into them, so they are kept until the context is destroyed instead of being freed.
     std::vector<void *> retired_scratch;
@@ -548,6 +552,46 @@ struct SampleArgs {
 };
 cudaError_t launch_sample(const SampleArgs &a, cudaStream_t s, uint64_t *launches);
 int32_t ensure_sampler_scratch(yule_cuda_ctx *ctx, size_t n_floats);
+
+// A batch of sequences served together.  `scratch` holds what the *_scratch_bytes function says; nothing is left in it from one call to the next.
+// Attention behind a shared prefix (prefix_attention.cu): the members are those of yule_prefix_attention, strides in floats and multiples of 4.
+struct PrefixAttention {
+    const float *q = nullptr, *prefix_k = nullptr, *prefix_v = nullptr, *tail_k = nullptr, *tail_v = nullptr;
+    const uint32_t *tail_lens = nullptr;
+    float *out = nullptr;
+    uint32_t hd = 0, n_heads = 0, n_kv_heads = 0, prefix_len = 0, n_seqs = 0, n_query = 1, tail_capacity = 0;
+    uint32_t q_stride = 0, out_stride = 0, prefix_stride = 0, tail_stride = 0;
+    void *scratch = nullptr;
+    bool pdl = false;
+};
+size_t prefix_attention_scratch_bytes(const PrefixAttention &a, int sm_count);
+cudaError_t launch_prefix_attention(const PrefixAttention &a, int sm_count, cudaStream_t s, uint64_t *launches);
+// Low-rank adapters (adapters.cu): the members are those of yule_adapters; n_cols and x_stride multiples of 4.
+struct AdapterBatch {
+    const void *down = nullptr, *up = nullptr;
+    const uint32_t *ranks = nullptr, *row_adapter = nullptr;
+    const float *scales = nullptr, *x = nullptr, *base = nullptr;
+    float *out = nullptr;
+    uint32_t type = 0, n_adapters = 0, max_rank = 0, n_rows = 0, n_cols = 0, batch = 0, x_stride = 0, out_stride = 0;
+    void *scratch = nullptr;
+    bool pdl = false;
+};
+size_t adapter_scratch_bytes(const AdapterBatch &a, int sm_count);
+cudaError_t launch_adapters(const AdapterBatch &a, int sm_count, cudaStream_t s, uint64_t *launches);
+// Verification of drafted tokens (verify.cu): the members are those of yule_verification; draft null: drafts without probabilities, lens null: n_draft each.
+struct VerifyDrafts {
+    const float *target = nullptr, *draft = nullptr;
+    const uint32_t *drafts = nullptr, *lens = nullptr;
+    const float *random = nullptr;
+    uint32_t *tokens = nullptr, *accepted = nullptr;
+    uint32_t vocab = 0, n_seqs = 0, n_draft = 0, target_stride = 0, draft_stride = 0;
+    float temperature = 1.f;
+    bool greedy = false;
+    void *scratch = nullptr;
+    bool pdl = false;
+};
+size_t verify_scratch_bytes(const VerifyDrafts &a);
+cudaError_t launch_verify_drafts(const VerifyDrafts &a, cudaStream_t s, uint64_t *launches);
 
 // Tiled 2-D tensor map (qgemm_tc.cu); `out` points to a CUtensorMap (128 bytes, 64-byte aligned).
 cudaError_t encode_tensor_map_2d(const void *base, uint32_t elem_bytes, uint64_t inner, uint64_t n_rows, uint64_t row_stride_bytes,
