@@ -1,5 +1,5 @@
 """Verification of drafted tokens (csrc/verify.cu) against its definition in 64 bits.  Tokens are whole numbers: they have to be equal.  The random numbers are drawn so that none lies
-within 2^-36 of a border (in units of the whole), far more than sums in 64 bits are off by."""
+within 2^-29 of a border (in units of the whole), more than the 2^-30 that its sums may be off by."""
 
 import numpy as np
 import pytest
@@ -100,7 +100,7 @@ class Call:
 
     def check(self, b):
         tokens, accepted, close = reference(self)
-        assert close > 2.0 ** -36, "a random number on a border says nothing"
+        assert close > 2.0 ** -29, "a random number on a border says nothing"
         got = self.got(b)
         assert (got[1] == accepted).all() and (got[0] == tokens).all()
         return accepted
@@ -195,6 +195,21 @@ def test_equal_distributions_accept_everything(backend):
     assert (c.check(backend) == 3).all()
 
 
+@pytest.mark.parametrize("V", [300, 50257])
+@pytest.mark.parametrize("step", [1e-2, 1e-4, 1e-6])
+def test_models_that_are_as_good_as_the_same(backend, V, step):
+    """Distributions that hardly differ, rejected all the same: all of w is where p and q are near.  (Half of the tokens a step more likely than drafted, half less.)"""
+    c = Call(B=6, K=2, V=V, temperature=1.0, spread=1.0)
+    r = np.random.default_rng(3)
+    c.target[:, :2] = np.round(c.target[:, :2] * 2 ** 10) / 2 ** 10
+    c.draft = (c.target[:, :2] + np.where(r.random((6, 2, V)) < 0.5, np.float32(step), np.float32(-step))).astype(np.float32)
+    for b in range(6):
+        c.drafts[b] = [np.nonzero(c.draft[b, t] > c.target[b, t])[0][0] for t in range(2)]
+    c.random[:, :2] = np.nextafter(np.float32(1), np.float32(0))
+    c.upload(backend).run(backend)
+    c.check(backend)
+
+
 def test_random_numbers_at_the_ends(backend):
     for u in (0.0, np.nextafter(np.float32(1), np.float32(0))):
         c = Call(B=8, K=3, V=300)
@@ -283,13 +298,13 @@ def test_refusals(backend):
     c.check(backend)
 
 
-def test_a_capture_cannot_grow_the_scratch():
+def test_first_call_in_a_capture():
+    """The call needs no scratch."""
     b = CudaB200Backend(0)
     c = Call().upload(b)
     b.graph_begin()
-    with pytest.raises(YuleGpuError, match="outside the capture"):
-        c.run(b)
-    b.graph_destroy(b.graph_end())
     c.run(b)
+    g = b.graph_end()
+    b.graph_launch(g)
     c.check(b)
     b.close()

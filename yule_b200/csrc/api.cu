@@ -1132,10 +1132,8 @@ int32_t yule_cuda_verify_drafts(yule_cuda_ctx *ctx, yule_buffer target_logits, y
     a.target = (const float *)T.ptr, a.drafts = (const uint32_t *)D.ptr, a.tokens = (uint32_t *)O.ptr, a.accepted = (uint32_t *)A.ptr;
     a.vocab = shape->vocab_size, a.n_seqs = shape->n_seqs, a.n_draft = shape->n_draft, a.target_stride = shape->target_stride, a.draft_stride = shape->draft_stride;
     a.temperature = shape->greedy ? 1.f : shape->temperature, a.greedy = shape->greedy != 0;
-    if (int32_t rc = ensure_batch_scratch(ctx, verify_scratch_bytes(a))) return rc;
-    a.scratch = ctx->batch_scratch;
     a.pdl = chain_goes_on(ctx, _chain.armed, _chain.n);
-    LAUNCHED(ctx, launch_verify_drafts(a, ctx->stream, &_n));
+    LAUNCHED(ctx, launch_verify_drafts(a, ctx->prop.multiProcessorCount, ctx->stream, &_n));
     chain_output(ctx, O.ptr, need.places);
     chain_output(ctx, A.ptr, need.of_seqs);
     ctx->pdl_chain = true;

@@ -587,11 +587,9 @@ struct VerifyDrafts {
     uint32_t vocab = 0, n_seqs = 0, n_draft = 0, target_stride = 0, draft_stride = 0;
     float temperature = 1.f;
     bool greedy = false;
-    void *scratch = nullptr;
     bool pdl = false;
 };
-size_t verify_scratch_bytes(const VerifyDrafts &a);
-cudaError_t launch_verify_drafts(const VerifyDrafts &a, cudaStream_t s, uint64_t *launches);
+cudaError_t launch_verify_drafts(const VerifyDrafts &a, int sm_count, cudaStream_t s, uint64_t *launches);
 
 // Tiled 2-D tensor map (qgemm_tc.cu); `out` points to a CUtensorMap (128 bytes, 64-byte aligned).
 cudaError_t encode_tensor_map_2d(const void *base, uint32_t elem_bytes, uint64_t inner, uint64_t n_rows, uint64_t row_stride_bytes,

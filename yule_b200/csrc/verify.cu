@@ -6,13 +6,21 @@
 // At the first that is not, place a, the token comes from w = max(0, p_a − q_a), after k accepted ones from w = p_k: the first i with Σ_{j <= i} w_j > u · Σ w, u the
 // last of the sequence's random numbers.  So the tokens are distributed as the target alone would give them.
 //
-// A pick next to a border has to be the same however the sums are formed, so exponentials and sums are in 64 bits: in 32 the running sum over 128256
-// tokens is off by 1e-7 where a token has 8e-6 on average, one pick in a hundred.
+// One launch, a cluster of CTAs per sequence, a slice of the vocabulary per CTA.  Places come in groups, each a pass over its rows of logits, one barrier of the
+// cluster and comparisons that all CTAs make alike: in a large batch the rows of a group behind the first rejected draft are not read and other sequences'
+// rows are on their way while one picks; in a small one all places are one group.
 //
-// Two kernels: largest logit and sum of exponentials of every row's chunks, a CTA each; then a cluster per sequence, which adds those up, compares, and sums w over a slice
-// of the vocabulary in each of its CTAs, in tiles, of which the one that holds the pick is gone through once more.
+// A pick next to a border has to be the same however the sums are formed: in 32 bits the running sum over 128256 tokens is off by 1e-7 where a token has 8e-6 on
+// average, one pick in a hundred.  So w and its sums are in 64 bits (exponentials to 2^-34, see Weight), for the two rows that the token is drawn from.  The
+// comparisons before it are in 32 bits, good to 2^-16, and made again in 64 where the two sides are nearer than 2^-13 of one another.
+//
+// w takes one pass over its two rows, although it needs the sums of both first: with the ratio of the sums known to 2^-16, tokens with p > q are told from the others,
+// and Σ w over them is Σ exp_p − ratio · Σ exp_q with the ratio known by then.  A token on the wrong side has |p − q| below 2^-16 of p, so with the mass of all
+// tokens that near at most 2^-14 of Σ w, w is good to 2^-30; with more (models that are as good as the same) a second pass knows the ratio.  The share of the
+// vocabulary that holds the pick is gone through again with w itself.
 
 #include <cfloat>
+#include <utility>
 
 #include <cooperative_groups.h>
 
@@ -24,242 +32,387 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr uint32_t kNothing = 0xFFFFFFFFu;
-constexpr uint32_t kCtas = 8;          // of a cluster
-constexpr uint32_t kTile = 4 * kThreads;  // tokens of a tile of the second kernel
+constexpr int kBatch = 16;           // logits of a row that a thread has on their way
+constexpr int kAhead = 4;            // and of the rows that it draws from
+constexpr float kNear = 0x1p-13f;
 
-struct RowPart {
-    double sum;   // of exp((logit − most) / temperature)
-    float most;   // −infinity: no token is possible
-    uint32_t at;  // the highest index of `most`
-};
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 struct VerifyParams {
     const float *target, *draft;
     const uint32_t *drafts, *lens;
     const float *random;
     uint32_t *tokens, *accepted;
-    RowPart *parts;  // [sequence][target rows, draft rows][chunk]
-    uint32_t vocab, n_seqs, n_draft, chunks;
+    uint32_t vocab, n_draft, group;
+    bool whole;  // rows begin on 16-byte boundaries
     size_t target_stride, draft_stride;
-    double inv_t;
-    bool greedy;
+    double per_bit;  // log2(e) / temperature
 };
 
 // A logit as it counts: NaN as −infinity, +infinity as the largest number.
-__device__ __forceinline__ float logit(const float *at) {
-    const float x = __ldg(at);
-    return x != x ? -INFINITY : fminf(x, FLT_MAX);
+__device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
+__device__ __forceinline__ float power(float x) {  // of two, to 2^-22; subnormal ones are nothing
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
-__device__ __forceinline__ double weight(float x, float most, double inv_t) { return exp(((double)x - (double)most) * inv_t); }
-__device__ __forceinline__ uint32_t rows_of(const VerifyParams &p) { return p.draft ? 2 * p.n_draft + 1 : p.n_draft + 1; }
-__device__ __forceinline__ uint32_t drafted(const VerifyParams &p, uint32_t b) { return p.lens ? min(__ldg(p.lens + b), p.n_draft) : p.n_draft; }
-__device__ __forceinline__ const float *target_row(const VerifyParams &p, uint32_t b, uint32_t t) { return p.target + ((size_t)b * (p.n_draft + 1) + t) * p.target_stride; }
-__device__ __forceinline__ const float *draft_row(const VerifyParams &p, uint32_t b, uint32_t t) { return p.draft + ((size_t)b * p.n_draft + t) * p.draft_stride; }
+
+// 2^((x − most) · per_bit) in 64 bits, for a logit x (clean or not) and the largest of its row, up to 2^-34 of itself; less than 2^-1022 is nothing.  Argument n + f, n rounded in 32 bits, |f| <= 0.501: 2^f by a polynomial of
+// degree 7 (interpolating at Chebyshev points), n into the exponent.  Nine operations in 64 bits, whose pipe bounds a pass over w.
+struct Weight {
+    double per_bit;
+    float most, per32, floor;  // floor: what lies below is nothing, and too far off to be rounded (rounded up: at most 1100 bits, or `most` itself)
+    __device__ __forceinline__ Weight(float m, double per) : per_bit(per), most(m), per32((float)per) { floor = __fsub_ru(m, (float)(1100.0 / per)); }
+    __device__ __forceinline__ double operator()(float x) const {
+        constexpr float kRound = 12582912.f;  // 1.5 · 2^23
+        const float c = fminf(fmaxf(x, floor), most), z = fmaf(c - most, per32, kRound);
+        const int n = __float_as_int(z) - 0x4B400000;
+        const double f = fma((double)c - (double)most, per_bit, -(double)(z - kRound));
+        double e = 1.530390509058455e-05;
+        e = fma(e, f, 0.0001546999476270236);
+        e = fma(e, f, 0.0013333477833756698);
+        e = fma(e, f, 0.009618024781872923);
+        e = fma(e, f, 0.05550410906806735);
+        e = fma(e, f, 0.24022651219745797);
+        e = fma(e, f, 0.6931471805567823);
+        e = fma(e, f, 0.9999999999589098);
+        const double w = __hiloint2double(__double2hiint(e) + (n << 20), __double2loint(e));
+        return !(x >= floor) || n < -1021 ? 0.0 : w;
+    }
+};
 
 // (most, at) of two: the larger, at equal size the higher index.
 __device__ __forceinline__ void take_larger(float &most, uint32_t &at, float other, uint32_t other_at) {
     if (other > most || (other == most && other_at > at)) most = other, at = other_at;
 }
-
-template <int N>  // tokens per thread
-__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const __grid_constant__ VerifyParams p) {
-    __shared__ float s_most[kThreads / 32];
-    __shared__ uint32_t s_at[kThreads / 32];
-    __shared__ double s_sum[kThreads / 32];
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t rows = rows_of(p), b = blockIdx.x / rows, r = blockIdx.x % rows, chunk = blockIdx.y, i0 = chunk * kThreads * N;
-    yule_pdl_launch_dependents();
-    yule_pdl_wait();
-    const uint32_t k = drafted(p, b);
-    const bool of_target = r <= p.n_draft;
-    const uint32_t t = of_target ? r : r - p.n_draft - 1;
-    if (of_target ? t > k : t >= k) return;
-    const float *row = of_target ? target_row(p, b, t) : draft_row(p, b, t);
-    float x[N], most = -INFINITY;
-    uint32_t at = 0;
+// A number's bits in an order that integers have.
+__device__ __forceinline__ int ordered(float x) {
+    const int i = __float_as_int(x);
+    return i ^ ((i >> 31) & 0x7FFFFFFF);
+}
+__device__ __forceinline__ float from_ordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7FFFFFFF)); }
+// (most, sum of 2^((x − most) · per_bit)) of a warp's lanes.
+__device__ __forceinline__ void join(float &most, float &sum, float per_bit) {
+    const float m = from_ordered(__reduce_max_sync(0xffffffffu, ordered(most)));
+    sum *= power((most - (m == -INFINITY ? 0.f : m)) * per_bit);
+    most = m;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const uint32_t j = i0 + i * kThreads + tid;
-        x[i] = j < p.vocab ? logit(row + j) : -INFINITY;
-    }
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const uint32_t j = i0 + i * kThreads + tid;
-        if (j < p.vocab) take_larger(most, at, x[i], j);
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) take_larger(most, at, __shfl_xor_sync(0xffffffffu, most, d), __shfl_xor_sync(0xffffffffu, at, d));
-    if (lane == 0) s_most[warp] = most, s_at[warp] = at;
-    __syncthreads();
-    most = s_most[0], at = s_at[0];
-#pragma unroll
-    for (int w = 1; w < kThreads / 32; w++) take_larger(most, at, s_most[w], s_at[w]);
-    double sum = 0.0;
-    if (!p.greedy && most != -INFINITY) {
-#pragma unroll
-        for (int i = 0; i < N; i++) sum += weight(x[i], most, p.inv_t);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (lane == 0) s_sum[warp] = sum;
-        __syncthreads();
-        sum = 0.0;
-        for (int w = 0; w < kThreads / 32; w++) sum += s_sum[w];
-    }
-    if (tid == 0) p.parts[((size_t)b * rows + r) * p.chunks + chunk] = RowPart{sum, most, at};
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
 }
 
-// Sum over the CTA, the same in every thread and every call.
-__device__ __forceinline__ double block_sum(double v, double *red) {
+// Over the lower sixteen lanes of a warp.
+__device__ __forceinline__ double sum16(double v) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0;
-    for (int w = 0; w < kThreads / 32; w++) v += red[w];
+    for (int d = 8; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
 }
+// Of sixteen parts in the lower lanes of a warp, the one in which the running sum (from `run` on) passes the goal, else the last that has anything (16: none); run: what is before it.
+__device__ __forceinline__ uint32_t part_of(double part, double goal, double &run) {
+    const uint32_t lane = threadIdx.x & 31;
+    part = lane < 16 && part > 0.0 ? part : 0.0;
+    double scan = part;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, scan, d);
+        if (lane >= (uint32_t)d) scan += x;
+    }
+    const uint32_t any = __ballot_sync(0xffffffffu, part > 0.0), past = __ballot_sync(0xffffffffu, part > 0.0 && run + scan > goal);
+    if (!any) return 16;
+    const uint32_t at = past ? __ffs(past) - 1 : 31 - __clz(any);
+    run += __shfl_sync(0xffffffffu, scan - part, at);
+    return at;
+}
 
-__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify_pick_kernel(const __grid_constant__ VerifyParams p) {
-    extern __shared__ __align__(16) unsigned char sm[];
+constexpr uint32_t kMostDrafts = 256;  // of a sequence (the entry point's limit)
+constexpr uint32_t kMostRows = 16;     // of a group
+
+struct Shared {
+    float2 row[2][16][kWarps];  // by parity of the group, CTA: what the warps have of their rows, written by them; greedy: (most, its index)
+    float2 whole[kMostRows];    // of the whole rows
+    uint32_t drafts[kMostDrafts];
+    float random[kMostDrafts], last_random, target_at[kMostDrafts], draft_at[kMostDrafts];  // logits of the drafts themselves; −infinity outside the vocabulary
+    double exact[2][5][16], warp_exact[5][kWarps];  // Σ exp_p, Σ exp_q; the same over tokens with p > q; Σ exp_p where the two are near; of the slices by parity of the pass
+    double warp_scan[kWarps];
+    uint32_t pick, last[kWarps];
+};
+
+template <int CTAS, bool GREEDY>
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_constant__ VerifyParams p) {
+    __shared__ Shared sh;
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t rank = cluster.block_rank(), b = blockIdx.x / kCtas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t rows = rows_of(p);
-    RowPart *row = reinterpret_cast<RowPart *>(sm);                 // [rows]
-    double *tile_sum = reinterpret_cast<double *>(row + rows);      // [tiles of a slice]
-    __shared__ double red[kThreads / 32], s_slice;
-    __shared__ uint32_t s_accepted, s_pick, s_last[kThreads / 32];
+    auto started = cluster.barrier_arrive();  // (waited for before anything is written to another CTA)
+    const uint32_t rank = blockIdx.x % CTAS, b = blockIdx.x / CTAS, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // a CTA's slice, and of it a warp's share
+    const uint32_t share = ((p.vocab + CTAS * kWarps - 1) / (CTAS * kWarps) + 3) & ~3u, lo = min(rank * kWarps * share, p.vocab), hi = min(lo + kWarps * share, p.vocab);
+    const float per_bit = (float)p.per_bit;
     yule_pdl_launch_dependents();
     yule_pdl_wait();
-    const uint32_t k = drafted(p, b);
-    for (uint32_t r = warp; r < rows; r += kThreads / 32) {
-        const uint32_t t = r <= p.n_draft ? r : r - p.n_draft - 1;
-        if (r <= p.n_draft ? t > k : t >= k) continue;
-        const RowPart *part = p.parts + ((size_t)b * rows + r) * p.chunks;
-        float most = -INFINITY;
-        uint32_t at = 0;
-        for (uint32_t c = lane; c < p.chunks; c += 32) take_larger(most, at, __ldcg(&part[c].most), __ldcg(&part[c].at));
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) take_larger(most, at, __shfl_xor_sync(0xffffffffu, most, d), __shfl_xor_sync(0xffffffffu, at, d));
-        double sum = 0.0;
-        for (uint32_t c = lane; c < p.chunks; c += 32) {
-            const float m = __ldcg(&part[c].most);
-            if (m != -INFINITY) sum += __ldcg(&part[c].sum) * weight(m, most, p.inv_t);
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (lane == 0) row[r] = RowPart{sum, most, at};
+    const uint32_t k = p.lens ? min(__ldg(p.lens + b), p.n_draft) : p.n_draft;
+    const float *target = p.target + (size_t)b * (p.n_draft + 1) * p.target_stride, *draft = !GREEDY && p.draft ? p.draft + (size_t)b * p.n_draft * p.draft_stride : nullptr;
+    for (uint32_t t = tid; t < k; t += kThreads) {
+        if (!GREEDY) sh.random[t] = __ldg(p.random + (size_t)b * (p.n_draft + 1) + t);
+        const uint32_t x = __ldg(p.drafts + (size_t)b * p.n_draft + t);
+        const bool in = x < p.vocab;
+        sh.drafts[t] = x;
+        sh.target_at[t] = in ? clean(__ldg(target + (size_t)t * p.target_stride + x)) : -INFINITY;
+        sh.draft_at[t] = in && draft ? clean(__ldg(draft + (size_t)t * p.draft_stride + x)) : -INFINITY;
     }
-    __syncthreads();
-    // what is accepted: a lane per draft
-    const uint32_t *drafts = p.drafts + (size_t)b * p.n_draft;
-    if (warp == 0) {
-        uint32_t accepted = 0;
-        for (uint32_t t0 = 0; t0 < k; t0 += 32) {
-            const uint32_t t = t0 + lane;
-            bool fits = true;
-            if (t < k) {
-                const uint32_t x = __ldg(drafts + t);
-                const RowPart pt = row[t];
-                if (x >= p.vocab || pt.most == -INFINITY) {
-                    fits = false;
-                } else if (p.greedy) {
-                    fits = pt.at == x;
-                } else {
-                    const double px = weight(logit(target_row(p, b, t) + x), pt.most, p.inv_t) / pt.sum;
-                    double qx = 1.0;
-                    if (p.draft) {
-                        const RowPart qt = row[p.n_draft + 1 + t];
-                        qx = qt.most == -INFINITY ? 0.0 : weight(logit(draft_row(p, b, t) + x), qt.most, p.inv_t) / qt.sum;
-                    }
-                    fits = (double)__ldg(p.random + (size_t)b * (p.n_draft + 1) + t) * qx < px;
-                }
-            }
-            const uint32_t no = __ballot_sync(0xffffffffu, !fits);
-            if (no) {
-                accepted = t0 + __ffs(no) - 1;
-                break;
-            }
-            accepted = min(k, t0 + 32);
-        }
-        if (lane == 0) s_accepted = accepted;
+    if (tid == 0) {
+        sh.pick = kNothing;
+        if (!GREEDY) sh.last_random = __ldg(p.random + (size_t)b * (p.n_draft + 1) + p.n_draft);
     }
-    if (tid == 0) s_pick = kNothing;
-    __syncthreads();
-    const uint32_t a = s_accepted;
-    const RowPart pa = row[a];
+    cluster.barrier_wait(std::move(started));
+
+    // Rows of a group are shared out to the warps: per_row of them a row, the target's rows of all places, then the draft model's.
+    const uint32_t kinds = draft ? 2 : 1, per_row = kWarps / (kinds * p.group), my_row = warp / per_row, place = my_row % p.group, kind = my_row / p.group;
+    const uint32_t first = (warp % per_row) * 32 + lane, step = per_row * 32;  // (of fours of logits, or of single ones)
+    uint32_t a = 0, g = p.group;  // the place in question, and which of its group it is
+    uint32_t t0 = 0u - p.group, parity = 0, pass = 0;
+    double z[5], ratio;
+    float pm, qm;
+    const float *pr, *qr;
     uint32_t *out = p.tokens + (size_t)b * (p.n_draft + 1);
     auto finish = [&](uint32_t pick) {  // by all threads of one CTA
-        for (uint32_t t = tid; t <= p.n_draft; t += kThreads) out[t] = t < a ? __ldg(drafts + t) : t == a ? pick : kNothing;
+        for (uint32_t t = tid; t <= p.n_draft; t += kThreads) out[t] = t < a ? sh.drafts[t] : t == a ? pick : kNothing;
         if (tid == 0) p.accepted[b] = a;
     };
-    if (p.greedy || pa.most == -INFINITY) {  // (the same for the whole cluster)
-        if (rank == 0) finish(pa.most == -INFINITY ? kNothing : pa.at);
-        return;
-    }
-    // w over this CTA's slice of the vocabulary, tile by tile
-    const float *pr = target_row(p, b, a), *qr = p.draft && a < k ? draft_row(p, b, a) : nullptr;
-    const RowPart qa = qr ? row[p.n_draft + 1 + a] : RowPart{1.0, -INFINITY, 0};
-    const uint32_t without = !p.draft && a < k ? __ldg(drafts + a) : kNothing;
-    const double inv_p = 1.0 / pa.sum, inv_q = 1.0 / qa.sum;
-    auto w_of = [&](uint32_t i) {
-        double w = weight(logit(pr + i), pa.most, p.inv_t) * inv_p;
-        if (qr && qa.most != -INFINITY) w -= weight(logit(qr + i), qa.most, p.inv_t) * inv_q;
-        return i == without || !(w > 0.0) ? 0.0 : w;
-    };
-    const uint32_t tiles = (p.vocab + kTile - 1) / kTile, per_cta = (tiles + kCtas - 1) / kCtas, tile0 = min(rank * per_cta, tiles), tile1 = min(tile0 + per_cta, tiles);
-    double slice = 0.0;
-    for (uint32_t j = tile0; j < tile1; j++) {
-        double w = 0.0;
+    for (;;) {
+        if (g == p.group) {
+            // The next group of places: largest logit and sum of exponentials of each row, in 32 bits.
+            t0 += p.group, g = 0, parity ^= 1u;
+            const uint32_t t = t0 + place;
+            float most = -INFINITY, sum = 0.f;
+            uint32_t at = 0;
+            if (kind == 0 ? t <= k : t < k) {
+                const float *row = kind == 0 ? target + (size_t)t * p.target_stride : draft + (size_t)t * p.draft_stride;
+                auto add = [&](float (&v)[kBatch], auto index) {
+                    if (GREEDY) {
 #pragma unroll
-        for (uint32_t e = 0; e < 4; e++) {
-            const uint32_t i = j * kTile + e * kThreads + tid;
-            if (i < p.vocab) w += w_of(i);
+                        for (int j = 0; j < kBatch; j++)
+                            if (index(j) < hi) take_larger(most, at, clean(v[j]), index(j));
+                        return;
+                    }
+                    float m = most;
+#pragma unroll
+                    for (int j = 0; j < kBatch; j++) m = fmaxf(m, v[j]);
+                    float from = m == -INFINITY ? 0.f : m;
+                    const uint64_t per2 = pair(per_bit, per_bit), from2 = pair(-from, -from);
+                    uint64_t sums2 = 0;
+#pragma unroll
+                    for (int j = 0; j < kBatch; j += 2) {
+                        const float2 e = unpair(mul2(add2(pair(v[j], v[j + 1]), from2), per2));
+                        sums2 = add2(sums2, pair(power(e.x), power(e.y)));
+                    }
+                    const float2 two = unpair(sums2);
+                    float s = fmaf(sum, power((most - from) * per_bit), two.x + two.y);
+                    if (!(s < INFINITY) || m == INFINITY) {  // NaN or infinity among them: once more, as they count
+                        m = most;
+#pragma unroll
+                        for (int j = 0; j < kBatch; j++) m = fmaxf(m, v[j] = clean(v[j]));
+                        from = m == -INFINITY ? 0.f : m;
+                        s = sum * power((most - from) * per_bit);
+                        for (int j = 0; j < kBatch; j++) s += power((v[j] - from) * per_bit);
+                    }
+                    most = m, sum = s;
+                };
+                float v[kBatch];
+                uint32_t i = lo + first;
+                if (p.whole) {
+                    for (i = lo + 4 * first; i + (kBatch - 4) * step + 4 <= hi; i += kBatch * step) {
+#pragma unroll
+                        for (int j = 0; j < kBatch; j += 4) {
+                            const float4 x = __ldg(reinterpret_cast<const float4 *>(row + i + j * step));
+                            v[j] = x.x, v[j + 1] = x.y, v[j + 2] = x.z, v[j + 3] = x.w;
+                        }
+                        add(v, [&](int j) { return i + (j & 3) + (j & ~3) * step; });
+                    }
+                    if (i < hi) {  // what is left
+                        auto index = [&](int j) { return i + (j & 3) + (j & ~3) * step; };
+#pragma unroll
+                        for (int j = 0; j < kBatch; j++) v[j] = index(j) < hi ? __ldg(row + index(j)) : -INFINITY;
+                        add(v, index);
+                    }
+                } else {
+                    for (; i < hi; i += kBatch * step) {
+#pragma unroll
+                        for (int j = 0; j < kBatch; j++) v[j] = i + j * step < hi ? __ldg(row + i + j * step) : -INFINITY;
+                        add(v, [&](int j) { return i + j * step; });
+                    }
+                }
+            }
+            if (GREEDY) {
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) take_larger(most, at, __shfl_xor_sync(0xffffffffu, most, d), __shfl_xor_sync(0xffffffffu, at, d));
+                sum = __uint_as_float(at);
+            } else {
+                join(most, sum, per_bit);
+            }
+            if (lane < CTAS) cluster.map_shared_rank(&sh, lane)->row[parity][rank][warp] = make_float2(most, sum);
+            cluster.sync();
+            // a warp per row
+            if (warp < kinds * p.group) {
+                most = -INFINITY, sum = 0.f, at = 0;
+                for (uint32_t i = lane; i < per_row * CTAS; i += 32) {
+                    const float2 o = sh.row[parity][i / per_row][warp * per_row + i % per_row];
+                    if (GREEDY) {
+                        take_larger(most, at, o.x, __float_as_uint(o.y));
+                    } else {
+                        const float m = fmaxf(most, o.x), from = m == -INFINITY ? 0.f : m;
+                        sum = sum * power((most - from) * per_bit) + o.y * power((o.x - from) * per_bit);
+                        most = m;
+                    }
+                }
+                if (GREEDY) {
+#pragma unroll
+                    for (int d = 16; d > 0; d >>= 1) take_larger(most, at, __shfl_xor_sync(0xffffffffu, most, d), __shfl_xor_sync(0xffffffffu, at, d));
+                    sum = __uint_as_float(at);
+                } else {
+                    join(most, sum, per_bit);
+                }
+                if (lane == 0) sh.whole[warp] = make_float2(most, sum);
+            }
+            __syncthreads();
         }
-        w = block_sum(w, red);
-        if (tid == 0) tile_sum[j - tile0] = w;
-        slice += w;
+        // Place t0 + g, by all threads alike.
+        a = t0 + g;
+        const float2 of_p = sh.whole[g], of_q = draft ? sh.whole[p.group + g] : make_float2(-INFINITY, 1.f);
+        pm = of_p.x, qm = of_q.x;
+        bool unsure = false;
+        if (a < k) {
+            bool fits = pm != -INFINITY && sh.target_at[a] != -INFINITY;
+            if (GREEDY) {
+                fits = fits && __float_as_uint(of_p.y) == sh.drafts[a];
+            } else if (fits) {
+                const float px = exp2f((sh.target_at[a] - pm) * per_bit) / of_p.y;
+                float ux = sh.random[a];
+                if (draft) ux *= qm == -INFINITY ? 0.f : exp2f((sh.draft_at[a] - qm) * per_bit) / of_q.y;
+                fits = ux < px * (1.f - kNear);
+                unsure = !fits && !(ux > px * (1.f + kNear));
+            }
+            if (fits) {
+                g++;
+                continue;
+            }
+        }
+        if (GREEDY || pm == -INFINITY) {
+            if (rank == 0) finish(pm == -INFINITY ? kNothing : __float_as_uint(of_p.y));
+            return;
+        }
+        // Not accepted, or too near to say, or the token behind the last draft: sums in 64 bits.
+        pr = target + (size_t)a * p.target_stride, qr = draft && a < k && qm != -INFINITY ? draft + (size_t)a * p.draft_stride : nullptr;
+        const uint32_t without = !draft && a < k ? sh.drafts[a] : kNothing;
+        ratio = qr ? (double)of_p.y / (double)of_q.y : 0.0;
+        for (bool known = !qr;;) {
+            const Weight wp(pm, p.per_bit), wq(qr ? qm : 0.f, p.per_bit);
+            double s0 = 0.0, s1 = 0.0, a0 = 0.0, a1 = 0.0, near = 0.0;
+            const uint32_t i1 = min(lo + (warp + 1) * share, hi);
+            float x[kAhead], y[kAhead];
+            auto load = [&](uint32_t i0) {
+#pragma unroll
+                for (int j = 0; j < kAhead; j++) {
+                    const uint32_t i = i0 + j * 32;
+                    x[j] = i < i1 ? __ldg(pr + i) : -INFINITY;
+                    y[j] = qr && i < i1 ? __ldg(qr + i) : -INFINITY;
+                }
+            };
+            load(lo + warp * share + lane);
+            for (uint32_t i0 = lo + warp * share + lane; i0 - lane < i1; i0 += kAhead * 32) {
+                float xs[kAhead], ys[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; j++) xs[j] = x[j], ys[j] = y[j];
+                load(i0 + kAhead * 32);
+#pragma unroll
+                for (int j = 0; j < kAhead; j++) {
+                const double e = wp(xs[j]);
+                    s0 += e;
+                    if (qr) {
+                        const double f = wq(ys[j]), d = fma(-ratio, f, e);
+                        s1 += f;
+                        const int of_d = __double2hiint(d);
+                        if (of_d >= 0) a0 += e, a1 += f;  // (a difference of zero adds nothing)
+                        if ((of_d & 0x7FF00000) <= (__double2hiint(e) & 0x7FF00000) - (15 << 20)) near += e;  // |d| < 2^-14 e, and all below 2^-16
+                    } else if (i0 + j * 32 != without) {
+                        a0 += e;
+                    }
+                }
+            }
+            double of[5] = {s0, s1, a0, a1, near};
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+                for (int i = 0; i < 5; i++) of[i] += __shfl_xor_sync(0xffffffffu, of[i], d);
+            if (lane == 0)
+#pragma unroll
+                for (int i = 0; i < 5; i++) sh.warp_exact[i][warp] = of[i];
+            __syncthreads();
+            pass++;
+            if (warp < 5) {
+                const double s = sum16(lane < kWarps ? sh.warp_exact[warp][lane] : 0.0);
+                if (lane < CTAS) cluster.map_shared_rank(&sh, lane)->exact[pass & 1u][warp][rank] = s;
+            }
+            cluster.sync();
+#pragma unroll
+            for (int i = 0; i < 5; i++) z[i] = __shfl_sync(0xffffffffu, sum16(lane < CTAS ? sh.exact[pass & 1u][i][lane] : 0.0), 0);
+            if (qr) ratio = z[0] / z[1];
+            if (known || !(z[4] > 0x1p-14 * (z[2] - ratio * z[3]))) break;
+            known = true;
+        }
+        if (unsure) {
+            const double px = Weight(pm, p.per_bit)(sh.target_at[a]) / z[0], qx = !draft ? 1.0 : qr ? Weight(qm, p.per_bit)(sh.draft_at[a]) / z[1] : 0.0;
+            if ((double)sh.random[a] * qx < px) {
+                g++;
+                continue;
+            }
+        }
+        break;
     }
-    if (tid == 0) s_slice = slice;
-    cluster.sync();
-    double total = 0.0, before = 0.0, mine = 0.0;
-    uint32_t owner = kCtas;
-    const double u = (double)__ldg(p.random + (size_t)b * (p.n_draft + 1) + p.n_draft);
-    double slices[kCtas];
-    for (uint32_t c = 0; c < kCtas; c++) total += slices[c] = *cluster.map_shared_rank(&s_slice, c);
-    const double goal = u * total;
-    for (uint32_t c = 0; c < kCtas; c++) {  // the slice in which the running sum passes the goal, else the last that has anything
-        if (!(slices[c] > 0.0)) continue;
-        owner = c, before = mine;
-        if (mine + slices[c] > goal) break;
-        mine += slices[c];
-    }
-    cluster.sync();  // (nobody leaves while its sum is read)
-    if (owner == kCtas) {
+
+    // The token: the slice of the vocabulary in which the running sum passes the goal, and in it the warp's share (every warp for itself).
+    const uint32_t without = !draft && a < k ? sh.drafts[a] : kNothing;
+    const double goal = (double)sh.last_random * (z[2] - ratio * z[3]);
+    double run = 0.0;
+    const uint32_t owner = part_of(lane < CTAS ? sh.exact[pass & 1u][2][lane] - ratio * sh.exact[pass & 1u][3][lane] : 0.0, goal, run);
+    if (owner == 16) {
         if (rank == 0) finish(kNothing);
         return;
     }
     if (rank != owner) return;
-    uint32_t at = tile0;
-    double run = before;
-    __syncthreads();
-    for (uint32_t j = tile0; j < tile1; j++) {
-        const double w = tile_sum[j - tile0];
-        if (!(w > 0.0)) continue;
-        at = j, before = run;
-        if (run + w > goal) break;
-        run += w;
-    }
-    // That tile again, four consecutive tokens a thread: the first whose running sum passes the goal, else the last that is possible.
-    double w[4], own = 0.0;
-    uint32_t last = kNothing;
-#pragma unroll
-    for (uint32_t e = 0; e < 4; e++) {
-        const uint32_t i = at * kTile + 4 * tid + e;
-        w[e] = i < p.vocab ? w_of(i) : 0.0;
-        own += w[e];
-        if (w[e] > 0.0) last = i;
+    const uint32_t of_warp = part_of(lane < kWarps ? sh.warp_exact[2][lane] - ratio * sh.warp_exact[3][lane] : 0.0, goal, run) & 15u;
+    // That share again, some consecutive tokens a thread: the first whose running sum passes the goal, else the last that is possible.
+    const Weight wp(pm, p.per_bit), wq(qr ? qm : 0.f, p.per_bit);
+    auto w_of = [&](uint32_t i) {
+        double w = wp(__ldg(pr + i));
+        if (qr) w = fma(-wq(__ldg(qr + i)), ratio, w);
+        return i == without || !(w > 0.0) ? 0.0 : w;
+    };
+    const uint32_t each = (share + kThreads - 1) / kThreads, s0 = min(lo + of_warp * share, hi), s1 = min(s0 + share, hi), i0 = min(s0 + tid * each, s1), i1 = min(i0 + each, s1);
+    double own = 0.0;
+    uint32_t last = 0;  // one more than its index
+    for (uint32_t i = i0; i < i1; i++) {
+        const double w = w_of(i);
+        own += w;
+        if (w > 0.0) last = i + 1;
     }
     double scan = own;
 #pragma unroll
@@ -267,54 +420,63 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kThreads) verify
         const double x = __shfl_up_sync(0xffffffffu, scan, d);
         if (lane >= (uint32_t)d) scan += x;
     }
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 31) sh.warp_scan[warp] = scan;
+    if (lane == 0) sh.last[warp] = last;
     __syncthreads();
-    if (lane == 31) red[warp] = scan;
-    uint32_t most = last == kNothing ? 0 : last + 1;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
-    if (lane == 0) s_last[warp] = most;
+    run += __shfl_sync(0xffffffffu, sum16(lane < warp ? sh.warp_scan[lane] : 0.0), 0) + (scan - own);
+    if (run + own > goal)
+        for (uint32_t i = i0; i < i1; i++) {
+            const double w = w_of(i);
+            run += w;
+            if (w > 0.0 && run > goal) {
+                atomicMin(&sh.pick, i);
+                break;
+            }
+        }
     __syncthreads();
-    double sum = before + (scan - own);
-    for (uint32_t v = 0; v < warp; v++) sum += red[v];
-    uint32_t pick = kNothing;
-#pragma unroll
-    for (uint32_t e = 0; e < 4; e++) {
-        sum += w[e];
-        if (pick == kNothing && w[e] > 0.0 && sum > goal) pick = at * kTile + 4 * tid + e;
-    }
-    if (pick != kNothing) atomicMin(&s_pick, pick);
-    __syncthreads();
-    if (s_pick == kNothing) {
-        pick = 0;
-        for (int v = 0; v < kThreads / 32; v++) pick = max(pick, s_last[v]);
-        finish(pick - 1);
-    } else {
-        finish(s_pick);
-    }
+    last = __reduce_max_sync(0xffffffffu, lane < kWarps ? sh.last[lane] : 0u);
+    finish(sh.pick != kNothing ? sh.pick : last - 1);
 }
 
-uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
-constexpr int kPerThread = 16;
+template <int CTAS, bool GREEDY>
+cudaError_t launch_variant(const VerifyParams &p, uint32_t n_seqs, bool pdl, cudaStream_t s) {
+    auto kern = verify_kernel<CTAS, GREEDY>;
+    if (CTAS > 8) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n_seqs * CTAS);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CTAS;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 2 : 1;
+    return launch_config(cfg, kern, p);
+}
 
 }  // namespace
 
-size_t verify_scratch_bytes(const VerifyDrafts &a) {
-    return (size_t)a.n_seqs * (a.draft ? 2 * a.n_draft + 1 : a.n_draft + 1) * ceil_div(a.vocab, kThreads * kPerThread) * sizeof(RowPart);
-}
-
-cudaError_t launch_verify_drafts(const VerifyDrafts &a, cudaStream_t s, uint64_t *launches) {
+cudaError_t launch_verify_drafts(const VerifyDrafts &a, int sm_count, cudaStream_t s, uint64_t *launches) {
     VerifyParams p = {};
     p.target = a.target, p.draft = a.draft, p.drafts = a.drafts, p.lens = a.lens, p.random = a.random, p.tokens = a.tokens, p.accepted = a.accepted;
-    p.parts = static_cast<RowPart *>(a.scratch);
-    p.vocab = a.vocab, p.n_seqs = a.n_seqs, p.n_draft = a.n_draft, p.chunks = ceil_div(a.vocab, kThreads * kPerThread);
-    p.target_stride = a.target_stride, p.draft_stride = a.draft_stride, p.inv_t = 1.0 / (double)a.temperature, p.greedy = a.greedy;
-    const uint32_t rows = a.draft ? 2 * a.n_draft + 1 : a.n_draft + 1;
-    if ((uint64_t)rows * a.n_seqs > 0x7FFFFFFFu || (uint64_t)a.n_seqs * kCtas > 0x7FFFFFFFu || p.chunks > 65535) return cudaErrorInvalidValue;
-    cudaError_t e = launch_kernel(verify_rows_kernel<kPerThread>, dim3(rows * a.n_seqs, p.chunks), dim3(kThreads), 0, s, a.pdl, p);
-    if (e != cudaSuccess) return e;
-    ++*launches;
-    const size_t smem = rows * sizeof(RowPart) + ceil_div(ceil_div(a.vocab, kTile), kCtas) * sizeof(double);
-    e = launch_kernel(verify_pick_kernel, dim3(a.n_seqs * kCtas), dim3(kThreads), smem, s, true, p);
+    p.vocab = a.vocab, p.n_draft = a.n_draft, p.target_stride = a.target_stride, p.draft_stride = a.draft_stride;
+    p.per_bit = 1.4426950408889634 / (double)a.temperature;
+    const bool few = (uint64_t)a.n_seqs * 16 <= 2 * (uint64_t)sm_count;
+    const uint32_t slice = a.vocab / (few ? 16 : 8) * 4 + 1, most = a.draft ? 8 : 16;
+    p.group = 1;
+    while (p.group < most && p.group * 2 * slice <= 65536 && p.group <= a.n_draft) p.group *= 2;
+    p.whole = a.target_stride % 4 == 0 && (!a.draft || a.draft_stride % 4 == 0);
+    if (const char *e = knob("YULE_VERIFY_GROUP")) p.group = atoi(e);
+    cudaError_t e;
+    if (few) e = a.greedy ? launch_variant<16, true>(p, a.n_seqs, a.pdl, s) : launch_variant<16, false>(p, a.n_seqs, a.pdl, s);
+    else e = a.greedy ? launch_variant<8, true>(p, a.n_seqs, a.pdl, s) : launch_variant<8, false>(p, a.n_seqs, a.pdl, s);
     if (e == cudaSuccess) ++*launches;
     return e;
 }
