@@ -112,6 +112,29 @@ def test_batches(backend, B):
     go(backend, B=B, H=8, kv=2, hd=64, P=300, C=40, seed=B)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("P", [64, 65, 95, 96, 97, 127, 128, 129, 200, 777, 4097, 20000])
+def test_many_rows(backend, hd, P):
+    """Enough query rows for 128 at a time: one tile of positions, several, a last one of few; rows that do not fill their 128."""
+    go(backend, B=11, T=1, H=8, kv=2, hd=hd, P=P, C=20, seed=P)
+    go(backend, B=45, T=2, H=3, kv=1, hd=hd, P=P, C=0, lens=np.zeros(45), seed=P)
+
+
+@pytest.mark.parametrize("where", ["pk", "pv"])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_a_prefix_that_is_not_finite(backend, where, value):
+    """Every row sees it: what is not finite in K makes no row finite, in V no row's dimension, and other KV heads are as they were."""
+    c = Call(B=20, H=8, kv=2, hd=128, P=300, C=20)
+    clean = reference(c.q, c.pk, c.pv, c.tk, c.tv, c.lens)
+    getattr(c, where)[150, 0, 5] = value
+    c.upload(backend).run(backend)
+    got = c.got(backend)
+    assert not np.isfinite(got[:, :, :4]).all(-1).any()
+    assert (np.abs(got - clean[0]).max(-1) <= clean[1])[:, :, 4:].all()
+    if where == "pv":
+        assert not np.isfinite(got[:, :, :4, 5]).any()
+
+
 def test_larger(backend):
     go(backend, B=32, H=32, kv=8, hd=128, P=2048, C=200, seed=1)
     go(backend, B=40, T=3, H=16, kv=2, hd=128, P=1111, C=99, seed=2)

@@ -1053,6 +1053,7 @@ int32_t yule_cuda_prefix_attention(yule_cuda_ctx *ctx, yule_buffer q, yule_buffe
     a.q_stride = shape->q_stride, a.out_stride = shape->out_stride, a.prefix_stride = shape->prefix_stride, a.tail_stride = shape->tail_stride;
     if (int32_t rc = ensure_batch_scratch(ctx, prefix_attention_scratch_bytes(a, ctx->prop.multiProcessorCount))) return rc;
     a.scratch = ctx->batch_scratch;
+    a.status = ctx->device_status;
     a.pdl = chain_goes_on(ctx, _chain.armed, _chain.n);
     LAUNCHED(ctx, launch_prefix_attention(a, ctx->prop.multiProcessorCount, ctx->stream, &_n));
     chain_output(ctx, O.ptr, need.out);

@@ -562,6 +562,7 @@ struct PrefixAttention {
     uint32_t hd = 0, n_heads = 0, n_kv_heads = 0, prefix_len = 0, n_seqs = 0, n_query = 1, tail_capacity = 0;
     uint32_t q_stride = 0, out_stride = 0, prefix_stride = 0, tail_stride = 0;
     void *scratch = nullptr;
+    int *status = nullptr;  // device status word for bounded waits
     bool pdl = false;
 };
 size_t prefix_attention_scratch_bytes(const PrefixAttention &a, int sm_count);

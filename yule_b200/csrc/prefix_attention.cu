@@ -12,7 +12,7 @@
 
 #include <cfloat>
 
-#include "internal.h"
+#include "prefix_attention.cuh"
 #include "tf32_common.cuh"
 
 namespace yule {
@@ -21,18 +21,6 @@ namespace {
 
 constexpr int kWarps = 4, kKeys = 16;  // a warp takes tiles of 16 positions in turn with the CTA's others
 constexpr uint32_t kTileKeys = kWarps * kKeys;
-
-struct PrefixParams {
-    const float *q, *prefix_k, *prefix_v, *tail_k, *tail_v;
-    const uint32_t *tail_lens;
-    float *out;
-    float2 *part_ml;  // [row][slot]: largest score (in units of ln 2), sum
-    float *part_o;    // [row][slot][hd]
-    uint32_t hd, n_heads, n_kv_heads, group, prefix_len, n_seqs, n_query, tail_capacity;
-    uint32_t prefix_splits, prefix_chunk, prefix_row_tiles, tail_splits, tail_chunk, tail_row_tiles, slots;
-    size_t q_stride, out_stride, prefix_stride, tail_stride;
-    float scale;
-};
 
 // Positions of sequence b's own caches (without capacity there are no lengths either).
 __device__ __forceinline__ uint32_t own_len(const PrefixParams &p, uint32_t b) { return p.tail_capacity ? min(__ldg(p.tail_lens + b), p.tail_capacity) : 0; }
@@ -60,8 +48,7 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
     uint32_t item = blockIdx.x, kvh, row0, n_rows, key0, key1, slot;
     const float *kc, *vc;
     size_t stride;
-    const uint32_t of_prefix = p.n_kv_heads * p.prefix_row_tiles * p.prefix_splits;
-    if (item < of_prefix) {
+    if (item < p.prefix_items) {
         slot = item % p.prefix_splits;
         item /= p.prefix_splits;
         kvh = item % p.n_kv_heads;
@@ -71,7 +58,7 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
         key1 = min(key0 + p.prefix_chunk, p.prefix_len);
         kc = p.prefix_k, vc = p.prefix_v, stride = p.prefix_stride;
     } else {
-        item -= of_prefix;
+        item -= p.prefix_items;
         const uint32_t split = item % p.tail_splits;
         item /= p.tail_splits;
         kvh = item % p.n_kv_heads;
@@ -333,41 +320,61 @@ cudaError_t launch_part(const PrefixParams &p, uint32_t items, bool pdl, cudaStr
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
-// The cut of the work: chunks such that the CTAs are a few per SM, of at least one tile for every warp.
-void shape_of(const PrefixAttention &a, int sm_count, PrefixParams *p, uint32_t *rows_in_eights) {
+// The cut of the work.
+struct Cut {
+    bool tc;        // the prefix goes to the kernel for 128 rows at a time
+    uint32_t rows;  // query rows of a CTA of the other one, in eights
+};
+Cut shape_of(const PrefixAttention &a, int sm_count, PrefixParams *p) {
     const uint32_t group = a.n_heads / a.n_kv_heads, mine = a.n_query * group, all = a.n_seqs * mine;
-    const uint32_t rows = *rows_in_eights = mine > 8 && a.hd <= 128 ? 2 : 1;
+    Cut cut;
+    cut.tc = prefix_tc_supported(a.hd) && all >= 32 && a.prefix_len >= 64;
+    if (const char *e = knob("YULE_PREFIX_TC")) cut.tc = prefix_tc_supported(a.hd) && atoi(e) != 0 && a.prefix_len > 0;
+    cut.rows = mine > 8 && a.hd <= 128 ? 2 : 1;
     p->group = group;
-    p->prefix_row_tiles = ceil_div(all, rows * 8);
-    p->tail_row_tiles = ceil_div(mine, rows * 8);
+    // Chunks such that the CTAs are a few per SM, of at least one tile for every warp.
     const uint32_t want = 4 * sm_count;
     auto chunk = [&](uint64_t units, uint32_t len) {
         const uint64_t per = units ? (want + units - 1) / units : 1;
         const uint64_t c = ((len + per - 1) / per + kTileKeys - 1) / kTileKeys * kTileKeys;
         return (uint32_t)(c < kTileKeys ? kTileKeys : c);
     };
-    p->prefix_chunk = chunk((uint64_t)a.n_kv_heads * p->prefix_row_tiles, a.prefix_len);
+    if (cut.tc) {
+        // One CTA per SM: rounds of them times the tiles of each, and what a round and a part to be added up cost.
+        p->prefix_row_tiles = ceil_div(all, kPrefixTcRows);
+        const uint64_t units = (uint64_t)a.n_kv_heads * p->prefix_row_tiles;
+        const uint32_t tiles = ceil_div(a.prefix_len, kPrefixTcKeys);
+        double least = 1e30;
+        for (uint32_t s = 1; s <= tiles && s <= 64; s++) {
+            const uint32_t each = ceil_div(tiles, s);
+            const double rounds = (double)((units * ceil_div(tiles, each) + sm_count - 1) / sm_count), cost = rounds * (4.0 + each) + 0.05 * s;
+            if (cost < least) least = cost, p->prefix_chunk = each * kPrefixTcKeys;
+        }
+    } else {
+        p->prefix_row_tiles = ceil_div(all, cut.rows * 8);
+        p->prefix_chunk = chunk((uint64_t)a.n_kv_heads * p->prefix_row_tiles, a.prefix_len);
+    }
     p->prefix_splits = ceil_div(a.prefix_len, p->prefix_chunk);
+    p->tail_row_tiles = ceil_div(mine, cut.rows * 8);
     const uint32_t common = a.tail_capacity > a.n_query - 1 ? a.tail_capacity - (a.n_query - 1) : 0;
     p->tail_chunk = chunk((uint64_t)a.n_kv_heads * a.n_seqs * p->tail_row_tiles, common);
     p->tail_splits = ceil_div(common, p->tail_chunk);
     p->slots = p->prefix_splits + p->tail_splits;
+    return cut;
 }
 
 }  // namespace
 
 size_t prefix_attention_scratch_bytes(const PrefixAttention &a, int sm_count) {
     PrefixParams p = {};
-    uint32_t rows;
-    shape_of(a, sm_count, &p, &rows);
+    shape_of(a, sm_count, &p);
     const size_t parts = (size_t)a.n_seqs * a.n_query * a.n_heads * p.slots;
     return parts * (sizeof(float2) + (size_t)a.hd * sizeof(float)) + 256;
 }
 
 cudaError_t launch_prefix_attention(const PrefixAttention &a, int sm_count, cudaStream_t s, uint64_t *launches) {
     PrefixParams p = {};
-    uint32_t rows;
-    shape_of(a, sm_count, &p, &rows);
+    const Cut cut = shape_of(a, sm_count, &p);
     p.q = a.q, p.prefix_k = a.prefix_k, p.prefix_v = a.prefix_v, p.tail_k = a.tail_k, p.tail_v = a.tail_v, p.tail_lens = a.tail_lens, p.out = a.out;
     p.hd = a.hd, p.n_heads = a.n_heads, p.n_kv_heads = a.n_kv_heads, p.prefix_len = a.prefix_len, p.n_seqs = a.n_seqs, p.n_query = a.n_query, p.tail_capacity = a.tail_capacity;
     p.q_stride = a.q_stride, p.out_stride = a.out_stride, p.prefix_stride = a.prefix_stride, p.tail_stride = a.tail_stride;
@@ -375,13 +382,20 @@ cudaError_t launch_prefix_attention(const PrefixAttention &a, int sm_count, cuda
     const size_t parts = (size_t)a.n_seqs * a.n_query * a.n_heads * p.slots;
     p.part_o = static_cast<float *>(a.scratch);
     p.part_ml = reinterpret_cast<float2 *>(p.part_o + parts * a.hd);
-    const uint64_t items = (uint64_t)p.n_kv_heads * p.prefix_row_tiles * p.prefix_splits + (uint64_t)a.n_seqs * p.n_kv_heads * p.tail_row_tiles * p.tail_splits;
+    p.status = a.status;
     const uint64_t out_rows = (uint64_t)a.n_seqs * a.n_query * a.n_heads;
+    uint64_t items = (uint64_t)a.n_seqs * p.n_kv_heads * p.tail_row_tiles * p.tail_splits;
+    if (!cut.tc) items += (uint64_t)p.n_kv_heads * p.prefix_row_tiles * p.prefix_splits;
     if (items > 0x7FFFFFFFu || out_rows > 0x7FFFFFFFu) return cudaErrorInvalidValue;
     cudaError_t e = cudaSuccess;
     bool pdl = a.pdl;
+    if (cut.tc) {
+        if ((e = launch_prefix_tc(p, pdl, s, launches)) != cudaSuccess) return e;
+        pdl = true;
+    }
+    p.prefix_items = cut.tc ? 0 : p.n_kv_heads * p.prefix_row_tiles * p.prefix_splits;
     if (items) {
-#define YULE_PART(H) e = rows == 1 ? launch_part<H, 1>(p, (uint32_t)items, pdl, s, launches) : launch_part<H, 2>(p, (uint32_t)items, pdl, s, launches)
+#define YULE_PART(H) e = cut.rows == 1 ? launch_part<H, 1>(p, (uint32_t)items, pdl, s, launches) : launch_part<H, 2>(p, (uint32_t)items, pdl, s, launches)
         if (a.hd <= 64) YULE_PART(64);
         else if (a.hd <= 96) YULE_PART(96);
         else if (a.hd <= 128) YULE_PART(128);

@@ -1,0 +1,26 @@
+// prefix_attention.cuh — what the kernels of the attention behind a shared prefix (prefix_attention.cu, prefix_attention_tc.cu) share.
+#pragma once
+
+#include "internal.h"
+
+namespace yule {
+
+struct PrefixParams {
+    const float *q, *prefix_k, *prefix_v, *tail_k, *tail_v;
+    const uint32_t *tail_lens;
+    float *out;
+    float2 *part_ml;  // [row][slot]: largest score (in units of ln 2), sum
+    float *part_o;    // [row][slot][hd]
+    uint32_t hd, n_heads, n_kv_heads, group, prefix_len, n_seqs, n_query, tail_capacity;
+    uint32_t prefix_splits, prefix_chunk, prefix_row_tiles, tail_splits, tail_chunk, tail_row_tiles, slots, prefix_items;
+    size_t q_stride, out_stride, prefix_stride, tail_stride;
+    float scale;  // log2(e) / sqrt(hd)
+    int *status;  // of bounded waits
+};
+
+// The prefix for 128 query rows at a time on tcgen05 (prefix_attention_tc.cu): leaves the parts of slots [0, prefix_splits).  prefix_chunk a multiple of 64; head_dim 64 or 128.
+constexpr uint32_t kPrefixTcRows = 128, kPrefixTcKeys = 64;
+bool prefix_tc_supported(uint32_t hd);
+cudaError_t launch_prefix_tc(const PrefixParams &p, bool pdl, cudaStream_t s, uint64_t *launches);
+
+}  // namespace yule
