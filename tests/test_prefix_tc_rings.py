@@ -1,5 +1,5 @@
-"""The hand-offs of the shared prefix on tcgen05 (csrc/prefix_attention_tc.cu) under random interleavings, on the CPU: one buffer of K operands, two of V, of scores and of
-probabilities by tile parity, waits that know a phase's parity only, MMAs that run in the order of their issue some time after it, and the words through which workers meet."""
+"""The hand-offs of the shared prefix on tcgen05 (csrc/prefix_attention_tc.cu) under random interleavings, on the CPU: one buffer of raw K and V and of K operands, two of V operands, of
+scores and of probabilities by tile parity, waits that know a phase's parity only, MMAs that run in the order of their issue some time after it, and the words through which workers meet."""
 
 import random
 
@@ -24,12 +24,13 @@ class Meeting:
         return lambda: self.over > mine
 
 
-def simulate(seed, n, s_wait=True, pv_wait=True, alpha_wait=True, inverses=4):
+def simulate(seed, n, s_wait=True, pv_wait=True, alpha_wait=True, raw_wait=True, inverses=4):
     rng = random.Random(seed)
     pair = lambda c: [Barrier(c), Barrier(c)]  # noqa: E731
     v_full, s_full, s_empty, p_full, pv_done, a_empty = pair(WORK), pair(1), pair(WORK), pair(WORK), pair(1), pair(SUM)
     k_full, o_full, o_empty, l_full = Barrier(WORK), Barrier(2), Barrier(SUM), Barrier(WORK)
     meet_k, meet_v, meet_rows = Meeting(WORK), Meeting(WORK), [Meeting(2) for _ in range(4)]
+    raw = {x: {"full": Barrier(1), "empty": Barrier(WORK), "is": -1, "read": [-1] * WORK} for x in "kv"}
     K, V, P = [None] * WORK, [[None] * WORK for _ in range(2)], [[None] * WORK for _ in range(2)]
     S, O, alpha, inverse = [None, None], None, [[None] * SUM for _ in range(2)], [None] * 4
     k_used, v_used, p_used, s_read, o_read, alpha_read, inverse_read = -1, {-1, -2}, {-1, -2}, [[-2 + b] * WORK for b in range(2)], [-1] * SUM, [[-2 + b] * SUM for b in range(2)], [-1] * SUM
@@ -51,14 +52,26 @@ def simulate(seed, n, s_wait=True, pv_wait=True, alpha_wait=True, inverses=4):
             assert most[which][at] == [j] * WORK, "a largest element of another tile"
             most_read[which][w] = j
 
-        def convert_k(j):
+        def read(x, j):
+            yield lambda: raw[x]["full"].over(j & 1)
+            assert raw[x]["is"] == j, "another tile's fp32 values"
+            yield lambda: True
+            assert raw[x]["is"] == j, "another tile's fp32 values"
+            raw[x]["read"][w] = j
+            raw[x]["empty"].arrive()
+
+        def read_k(j):
+            yield from read("k", j)
             yield from largest("k", meet_k, j)
+
+        def store_k(j):
             assert k_used >= j - 1, "K overwritten before its scores"
             K[w] = j
             yield lambda: True
             k_full.arrive()
 
         def convert_v(j):
+            yield from read("v", j)
             yield from largest("v", meet_v, j)
             if pv_wait:
                 yield lambda: pv_done[j & 1].over(j // 2 & 1 ^ 1)
@@ -70,15 +83,22 @@ def simulate(seed, n, s_wait=True, pv_wait=True, alpha_wait=True, inverses=4):
             yield lambda: True
             v_full[j & 1].arrive()
 
-        yield from convert_k(0)
+        yield from read_k(0)
+        yield from store_k(0)
         yield from convert_v(0)
         for j in range(n):
             b, ph = j & 1, j >> 1 & 1
+            if j + 1 < n:
+                yield from read_k(j + 1)
             if s_wait:
                 yield lambda: s_full[b].over(ph)
             if j + 1 < n:
-                yield from convert_k(j + 1)
+                yield from store_k(j + 1)
             assert S[b] == j, "scores of another tile"
+            yield lambda: True
+            assert S[b] == j
+            s_read[b][w] = j
+            s_empty[b].arrive()
             other = rows_read[quarter][half ^ 1]
             assert other >= j - 2, "a row's word overwritten before it was read"
             rows[quarter][b][half] = j
@@ -90,9 +110,6 @@ def simulate(seed, n, s_wait=True, pv_wait=True, alpha_wait=True, inverses=4):
             if half == 0:
                 assert alpha_read[b][quarter] >= j - 2, "alpha overwritten before it was read"
                 alpha[b][quarter] = j
-            assert S[b] == j
-            s_read[b][w] = j
-            s_empty[b].arrive()
             yield lambda: True
             assert j - 2 in p_used, "probabilities overwritten before they were used"
             P[b][w] = j
@@ -100,6 +117,22 @@ def simulate(seed, n, s_wait=True, pv_wait=True, alpha_wait=True, inverses=4):
             if j + 1 < n:
                 yield from convert_v(j + 1)
         l_full.arrive()
+
+    def loader():
+        def copy(x, j):
+            def go():
+                assert raw[x]["read"] == [j - 1] * WORK, "fp32 values overwritten before they were read"
+                raw[x]["is"] = j
+            return go
+
+        for j in range(n):
+            for x in "kv":
+                if raw_wait:
+                    yield lambda: raw[x]["empty"].over(j & 1 ^ 1)
+                copies[x].extend([copy(x, j), raw[x]["full"].arrive])
+                yield lambda: True
+
+    copies = {"k": [], "v": []}
 
     def issue():
         def scores(j):
@@ -148,7 +181,7 @@ def simulate(seed, n, s_wait=True, pv_wait=True, alpha_wait=True, inverses=4):
             o_empty.arrive()
         yield lambda: l_full.over(0)
 
-    interleave(rng, [issue()] + [worker(w) for w in range(WORK)] + [sums(w) for w in range(SUM)], [queue])
+    interleave(rng, [issue(), loader()] + [worker(w) for w in range(WORK)] + [sums(w) for w in range(SUM)], [queue, *copies.values()])
 
 
 @pytest.mark.parametrize("n", [1, 2, 3, 4, 9, 14])
@@ -157,7 +190,7 @@ def test_hand_offs_hold(n):
         simulate(seed, n)
 
 
-@pytest.mark.parametrize("missing", [dict(s_wait=False), dict(pv_wait=False), dict(alpha_wait=False), dict(inverses=1)])
+@pytest.mark.parametrize("missing", [dict(s_wait=False), dict(pv_wait=False), dict(alpha_wait=False), dict(raw_wait=False), dict(inverses=1)])
 def test_the_model_catches_what_is_missing(missing):
     with pytest.raises(AssertionError):
         for seed in range(400):
