@@ -254,8 +254,8 @@ int32_t yule_cuda_embed_gather(yule_cuda_ctx *ctx, yule_buffer table, uint32_t g
  * tail_stride apart.  tail_lens: n_seqs words, the positions that sequence b's own caches hold, its query tokens' among them (the newest n_query; more than
  * tail_capacity counts as tail_capacity): query token t sees its own and earlier ones, tail_lens[b] - (n_query - 1 - t) positions, none if that is negative.
  * A row that sees nothing is zero.  Scores, soft-max and head grouping as yule_cuda_multihead_attention.  Handles of a prefix_len
- * or tail_capacity of 0 are not looked at.  A value that is not finite in a position that a row sees makes that row's output not finite; what no
- * row of a sequence sees is not read.  head_dim a multiple of 4, at most 256; strides multiples of 4; n_query at most 64. */
+ * or tail_capacity of 0 are not looked at.  A value that is not finite in a position that a row sees makes that row's output not finite; what a
+ * row does not see does not count for it, whatever it holds.  head_dim a multiple of 4, at most 256; strides multiples of 4; n_query at most 64. */
 typedef struct yule_prefix_attention {
     uint32_t head_dim, n_heads, n_kv_heads;
     uint32_t prefix_len, n_seqs, n_query, tail_capacity;

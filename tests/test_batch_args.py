@@ -74,7 +74,7 @@ def test_bytes_of_prefix_attention(checks):
     (dict(n_heads=0), "shape"), (dict(n_kv_heads=0), "shape"), (dict(n_heads=30), "shape"), (dict(n_seqs=0), "shape"), (dict(head_dim=0), "head_dim"),
     (dict(head_dim=130), "head_dim"), (dict(head_dim=260), "head_dim"), (dict(n_query=0), "query"), (dict(n_query=65), "query"), (dict(q_stride=4092), "strides"),
     (dict(out_stride=4092), "strides"), (dict(prefix_stride=1020), "strides"), (dict(tail_stride=1020), "strides"), (dict(q_stride=4097), "strides"),
-    (dict(out_stride=4098), "strides"), (dict(prefix_stride=1025), "strides"), (dict(tail_stride=1030), "strides"), (dict(n_seqs=0xFFFFFFFF), "rows"),
+    (dict(out_stride=4098), "strides"), (dict(prefix_stride=1025), "strides"), (dict(tail_stride=1030), "strides"), (dict(n_seqs=0xFFFFFFFF), "positions"), (dict(n_seqs=0xFFFFFFFF, tail_capacity=0), "rows"),
     (dict(prefix_len=0x80000000), "positions"), (dict(tail_capacity=0xFFFFFFFF), "positions")])
 def test_refusals_of_prefix_attention(checks, over, word):
     rc, _, said = asked(checks, "prefix", prefix(**over))
@@ -82,7 +82,7 @@ def test_refusals_of_prefix_attention(checks, over, word):
 
 
 def test_products_do_not_come_out_small(checks):
-    for kind, shape in (("prefix", prefix(n_seqs=1 << 24, tail_capacity=0x7FFFFFFF, tail_stride=0xFFFFFFFC)), ("adapters", adapters(n_adapters=0xFFFFFFFF, n_cols=0xFFFFFFFC, x_stride=0xFFFFFFFC)),
+    for kind, shape in (("prefix", prefix(n_seqs=1 << 12, n_heads=8, tail_capacity=0x7FFFF, tail_stride=0xFFFFFFFC)), ("adapters", adapters(n_adapters=0xFFFFFFFF, n_cols=0xFFFFFFFC, x_stride=0xFFFFFFFC)),
                         ("verification", verification(target_stride=0xFFFFFFFF, n_seqs=65536, n_draft=256))):
         rc, need, _ = asked(checks, kind, shape)
         assert rc == 0 and max(need) >= 1 << 56

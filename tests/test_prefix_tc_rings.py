@@ -1,5 +1,5 @@
-"""The hand-offs of the shared prefix on tcgen05 (csrc/prefix_attention_tc.cu) under random interleavings, on the CPU: one buffer of raw K and V and of K operands, two of V operands, of
-scores and of probabilities by tile parity, waits that know a phase's parity only, MMAs that run in the order of their issue some time after it, and the words through which workers meet."""
+"""The hand-offs of the shared prefix on tcgen05 (csrc/prefix_attention_tc.cu) under random interleavings, on the CPU: three buffers of K, two of V, of scores and of
+probabilities by tile parity, waits that know a phase's parity only, MMAs and copies that run in the order of their issue some time after it, and the words through which the halves of a row meet."""
 
 import random
 
@@ -7,7 +7,7 @@ import pytest
 
 from interleavings import Barrier, interleave
 
-WORK, SUM = 8, 4
+SOFT, SUM = 8, 4
 
 
 class Meeting:
@@ -24,155 +24,106 @@ class Meeting:
         return lambda: self.over > mine
 
 
-def simulate(seed, n, s_wait=True, pv_wait=True, alpha_wait=True, raw_wait=True, inverses=4):
+def simulate(seed, n, k_wait=True, v_wait=True, alpha_wait=True, s_wait=True, o_wait=True):
     rng = random.Random(seed)
     pair = lambda c: [Barrier(c), Barrier(c)]  # noqa: E731
-    v_full, s_full, s_empty, p_full, pv_done, a_empty = pair(WORK), pair(1), pair(WORK), pair(WORK), pair(1), pair(SUM)
-    k_full, o_full, o_empty, l_full = Barrier(WORK), Barrier(2), Barrier(SUM), Barrier(WORK)
-    meet_k, meet_v, meet_rows = Meeting(WORK), Meeting(WORK), [Meeting(2) for _ in range(4)]
-    raw = {x: {"full": Barrier(1), "empty": Barrier(WORK), "is": -1, "read": [-1] * WORK} for x in "kv"}
-    K, V, P = [None] * WORK, [[None] * WORK for _ in range(2)], [[None] * WORK for _ in range(2)]
-    S, O, alpha, inverse = [None, None], None, [[None] * SUM for _ in range(2)], [None] * 4
-    k_used, v_used, p_used, s_read, o_read, alpha_read, inverse_read = -1, {-1, -2}, {-1, -2}, [[-2 + b] * WORK for b in range(2)], [-1] * SUM, [[-2 + b] * SUM for b in range(2)], [-1] * SUM
-    most = {"k": [[None] * WORK for _ in range(2)], "v": [[None] * WORK for _ in range(2)]}
-    most_read = {"k": [-1] * WORK, "v": [-1] * WORK}
+    k_full, k_empty = [Barrier(1) for _ in range(3)], [Barrier(1) for _ in range(3)]
+    v_full, v_empty, s_full, s_empty, p_full, a_empty = pair(1), pair(1), pair(1), pair(SOFT), pair(SOFT), pair(SUM)
+    o_full, o_empty, l_full = Barrier(2), Barrier(SUM), Barrier(SOFT)
+    meet_rows = [Meeting(2) for _ in range(4)]
+    K, V, S, P, O = [None] * 3, [None] * 2, [None] * 2, [[None] * SOFT for _ in range(2)], None
+    alpha = [[None] * SUM for _ in range(2)]
+    k_used, v_used, p_used, s_read, o_read, alpha_read = {-1, -2, -3}, {-1, -2}, {-1, -2}, [[-2 + b] * SOFT for b in range(2)], [-1] * SUM, [[-2 + b] * SUM for b in range(2)]
     rows, rows_read = [[[None] * 2 for _ in range(2)] for _ in range(4)], [[-1] * 2 for _ in range(4)]
-    queue = []
+    queue, copies = [], []
 
-    def worker(w):
-        quarter, half = w & 3, w >> 2
+    def loader():
+        def copy(to, used, j):
+            def go():
+                assert j - len(to) in used, "an operand overwritten before it was used"
+                to[j % len(to)] = j
+            return go
 
-        def largest(which, meeting, j):
-            at = j & 1
-            assert min(most_read[which]) >= j - 2, "a word overwritten before it was read"
-            most[which][at][w] = j
-            yield meeting.meet()
-            assert most[which][at] == [j] * WORK, "a largest element of another tile"
-            yield lambda: True
-            assert most[which][at] == [j] * WORK, "a largest element of another tile"
-            most_read[which][w] = j
-
-        def read(x, j):
-            yield lambda: raw[x]["full"].over(j & 1)
-            assert raw[x]["is"] == j, "another tile's fp32 values"
-            yield lambda: True
-            assert raw[x]["is"] == j, "another tile's fp32 values"
-            raw[x]["read"][w] = j
-            raw[x]["empty"].arrive()
-
-        def read_k(j):
-            yield from read("k", j)
-            yield from largest("k", meet_k, j)
-
-        def store_k(j):
-            assert k_used >= j - 1, "K overwritten before its scores"
-            K[w] = j
-            yield lambda: True
-            k_full.arrive()
-
-        def convert_v(j):
-            yield from read("v", j)
-            yield from largest("v", meet_v, j)
-            if pv_wait:
-                yield lambda: pv_done[j & 1].over(j // 2 & 1 ^ 1)
-            assert j - 2 in v_used, "V overwritten before it was used"
-            V[j & 1][w] = j
-            if w == 0:
-                assert min(inverse_read) >= j - inverses, "an inverse scale overwritten before it was read"
-                inverse[j % inverses] = j
-            yield lambda: True
-            v_full[j & 1].arrive()
-
-        yield from read_k(0)
-        yield from store_k(0)
-        yield from convert_v(0)
+        for j in range(min(2, n)):
+            copies.extend([copy(K, k_used, j), k_full[j].arrive])
         for j in range(n):
             b, ph = j & 1, j >> 1 & 1
-            if j + 1 < n:
-                yield from read_k(j + 1)
-            if s_wait:
-                yield lambda: s_full[b].over(ph)
-            if j + 1 < n:
-                yield from store_k(j + 1)
+            if v_wait:
+                yield lambda: v_empty[b].over(ph ^ 1)
+            copies.extend([copy(V, v_used, j), v_full[b].arrive])
+            i = j + 2
+            if i < n:
+                if k_wait:
+                    yield lambda: k_empty[i % 3].over(i // 3 & 1 ^ 1)
+                copies.extend([copy(K, k_used, i), k_full[i % 3].arrive])
+            yield lambda: True
+
+    def softmax(w):
+        quarter, half = w & 3, w >> 2
+        for j in range(n):
+            b, ph = j & 1, j >> 1 & 1
+            if alpha_wait:
+                yield lambda: a_empty[b].over(ph ^ 1)
+            yield lambda: s_full[b].over(ph)
             assert S[b] == j, "scores of another tile"
             yield lambda: True
-            assert S[b] == j
+            assert S[b] == j, "scores of another tile"
             s_read[b][w] = j
             s_empty[b].arrive()
-            other = rows_read[quarter][half ^ 1]
-            assert other >= j - 2, "a row's word overwritten before it was read"
+            assert rows_read[quarter][half ^ 1] >= j - 2, "a row's word overwritten before it was read"
             rows[quarter][b][half] = j
             yield meet_rows[quarter].meet()
             assert rows[quarter][b][half ^ 1] == j, "another tile's largest score"
             rows_read[quarter][half] = j
-            if alpha_wait:
-                yield lambda: a_empty[b].over(ph ^ 1)
             if half == 0:
                 assert alpha_read[b][quarter] >= j - 2, "alpha overwritten before it was read"
                 alpha[b][quarter] = j
-            yield lambda: True
             assert j - 2 in p_used, "probabilities overwritten before they were used"
             P[b][w] = j
+            yield lambda: True
             p_full[b].arrive()
-            if j + 1 < n:
-                yield from convert_v(j + 1)
         l_full.arrive()
-
-    def loader():
-        def copy(x, j):
-            def go():
-                assert raw[x]["read"] == [j - 1] * WORK, "fp32 values overwritten before they were read"
-                raw[x]["is"] = j
-            return go
-
-        for j in range(n):
-            for x in "kv":
-                if raw_wait:
-                    yield lambda: raw[x]["empty"].over(j & 1 ^ 1)
-                copies[x].extend([copy(x, j), raw[x]["full"].arrive])
-                yield lambda: True
-
-    copies = {"k": [], "v": []}
 
     def issue():
         def scores(j):
             def go():
-                nonlocal k_used
                 b = j & 1
-                assert K == [j] * WORK, "scores of another tile's K"
-                assert s_read[b] == [j - 2] * WORK, "scores overwritten before they were read"
-                S[b], k_used = j, j
+                assert K[j % 3] == j, "scores of another tile's K"
+                assert s_read[b] == [j - 2] * SOFT, "scores overwritten before they were read"
+                S[b] = j
+                k_used.add(j)
             return go
 
         def output(j):
             def go():
                 nonlocal O
-                assert V[j & 1] == [j] * WORK and P[j & 1] == [j] * WORK, "output of other operands"
+                assert V[j & 1] == j and P[j & 1] == [j] * SOFT, "output of other operands"
                 assert o_read == [j - 1] * SUM, "output overwritten before it was read"
                 O = j
                 v_used.add(j)
                 p_used.add(j)
             return go
 
-        for j in range(-1, n):
-            if j + 1 < n:
-                i = j + 1
-                yield lambda: s_empty[i & 1].over(i >> 1 & 1 ^ 1)
-                yield lambda: k_full.over(i & 1)
-                queue.extend([scores(i), s_full[i & 1].arrive])
+        for j in range(-2, n):
+            if j + 2 < n:
+                i = j + 2
+                if s_wait:
+                    yield lambda: s_empty[i & 1].over(i >> 1 & 1 ^ 1)
+                yield lambda: k_full[i % 3].over(i // 3 & 1)
+                queue.extend([scores(i), k_empty[i % 3].arrive, s_full[i & 1].arrive])
             if j >= 0:
                 b, ph = j & 1, j >> 1 & 1
                 yield lambda: v_full[b].over(ph)
-                yield lambda: o_empty.over(j & 1 ^ 1)
+                if o_wait:
+                    yield lambda: o_empty.over(j & 1 ^ 1)
                 yield lambda: p_full[b].over(ph)
-                queue.extend([output(j), o_full.arrive, pv_done[b].arrive])
+                queue.extend([output(j), v_empty[b].arrive, o_full.arrive])
                 o_full.arrive()
 
     def sums(w):
         for j in range(n):
             yield lambda: o_full.over(j & 1)
-            assert O == j and alpha[j & 1][w] == j and inverse[j % inverses] == j, "output, alpha or scale of another tile"
-            inverse_read[w] = j
+            assert O == j and alpha[j & 1][w] == j, "output or alpha of another tile"
             alpha_read[j & 1][w] = j
             a_empty[j & 1].arrive()
             yield lambda: True
@@ -180,8 +131,9 @@ def simulate(seed, n, s_wait=True, pv_wait=True, alpha_wait=True, raw_wait=True,
             o_read[w] = j
             o_empty.arrive()
         yield lambda: l_full.over(0)
+        assert k_used >= set(range(n)) and v_used >= set(range(n)) and not queue and not copies, "the operands' memory taken while they are in use"
 
-    interleave(rng, [issue(), loader()] + [worker(w) for w in range(WORK)] + [sums(w) for w in range(SUM)], [queue, *copies.values()])
+    interleave(rng, [issue(), loader()] + [softmax(w) for w in range(SOFT)] + [sums(w) for w in range(SUM)], [queue, copies])
 
 
 @pytest.mark.parametrize("n", [1, 2, 3, 4, 9, 14])
@@ -190,8 +142,8 @@ def test_hand_offs_hold(n):
         simulate(seed, n)
 
 
-@pytest.mark.parametrize("missing", [dict(s_wait=False), dict(pv_wait=False), dict(alpha_wait=False), dict(raw_wait=False), dict(inverses=1)])
+@pytest.mark.parametrize("missing", ["k_wait", "v_wait", "alpha_wait", "s_wait", "o_wait"])
 def test_the_model_catches_what_is_missing(missing):
     with pytest.raises(AssertionError):
         for seed in range(400):
-            simulate(seed, 9, **missing)
+            simulate(seed, 9, **{missing: False})

@@ -29,11 +29,12 @@ struct PrefixNeeds {
 inline int32_t check_prefix_attention(const yule_prefix_attention *shape, PrefixNeeds *need) {
     if (!shape) return fail(YULE_ERR_INVALID_ARGUMENT, "null shape");
     const yule_prefix_attention &s = *shape;
-    if (s.n_kv_heads == 0 || s.n_heads == 0 || s.n_heads % s.n_kv_heads || s.n_seqs == 0)
+    if (s.n_kv_heads == 0 || s.n_kv_heads > 65535 || s.n_heads == 0 || s.n_heads % s.n_kv_heads || s.n_seqs == 0)
         return fail(YULE_ERR_INVALID_ARGUMENT, "bad attention shape (heads %u, kv heads %u, sequences %u)", s.n_heads, s.n_kv_heads, s.n_seqs);
     if (s.head_dim == 0 || s.head_dim % 4 || s.head_dim > 256) return fail(YULE_ERR_INVALID_ARGUMENT, "head_dim %u must be a multiple of 4 and at most 256", s.head_dim);
     if (s.n_query == 0 || s.n_query > 64) return fail(YULE_ERR_INVALID_ARGUMENT, "%u query tokens per sequence: from 1 to 64", s.n_query);
-    if (s.prefix_len > 0x7FFFFFFFu || s.tail_capacity > 0x7FFFFFFFu) return fail(YULE_ERR_INVALID_ARGUMENT, "at most 2^31 - 1 positions");
+    if (s.prefix_len > 0x7FFFFFFFu || times(s.n_seqs, s.tail_capacity) > 0x7FFFFFFFu)
+        return fail(YULE_ERR_INVALID_ARGUMENT, "at most 2^31 - 1 positions of the prefix, and of all sequences' own caches together");
     const uint64_t heads = (uint64_t)s.n_heads * s.head_dim, kv = (uint64_t)s.n_kv_heads * s.head_dim, tokens = (uint64_t)s.n_seqs * s.n_query;
     if (s.q_stride < heads || s.out_stride < heads || (s.prefix_len && s.prefix_stride < kv) || (s.tail_capacity && s.tail_stride < kv) || s.q_stride % 4 || s.out_stride % 4 ||
         s.prefix_stride % 4 || s.tail_stride % 4)

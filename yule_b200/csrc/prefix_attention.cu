@@ -10,20 +10,27 @@
 // with them the at most n_query − 1 newest positions that not all query tokens see, one by one in fp32 (so that what is hidden from a row is not read for it).
 // Parts are added in a fixed order: the same call gives the same bits.
 
+#include <cuda.h>
+
 #include <cfloat>
 
 #include "prefix_attention.cuh"
+#include "qgemm_common.cuh"
 #include "tf32_common.cuh"
 
 namespace yule {
 
 namespace {
 
-constexpr int kWarps = 4, kKeys = 16;  // a warp takes tiles of 16 positions in turn with the CTA's others
+constexpr int kWarps = 2, kKeys = 16;  // a warp takes tiles of 16 positions in turn with the CTA's other
 constexpr uint32_t kTileKeys = kWarps * kKeys;
 
+struct PartMaps {
+    CUtensorMap m[4];  // prefix K and V, own K and V: rows in boxes of 16 positions by 32 dimensions, swizzled within 128 bytes
+};
+
 // Positions of sequence b's own caches (without capacity there are no lengths either).
-__device__ __forceinline__ uint32_t own_len(const PrefixParams &p, uint32_t b) { return p.tail_capacity ? min(__ldg(p.tail_lens + b), p.tail_capacity) : 0; }
+__device__ __forceinline__ uint32_t own_len(const PrefixParams &p, uint32_t b) { return p.tail_capacity ? min(__ldcg(p.tail_lens + b), p.tail_capacity) : 0; }
 // Positions of sequence b that all its query tokens see.
 __device__ __forceinline__ uint32_t common_len(const PrefixParams &p, uint32_t b) {
     const uint32_t n = own_len(p, b);
@@ -32,49 +39,71 @@ __device__ __forceinline__ uint32_t common_len(const PrefixParams &p, uint32_t b
 __device__ __forceinline__ float4 load4(const float *at, bool there) { return there ? __ldcg(reinterpret_cast<const float4 *>(at)) : make_float4(0.f, 0.f, 0.f, 0.f); }
 
 // A warp per tile of 16 positions, the positions as rows of the tensor core's first operand and the query rows as the eight columns of its second, so that a CTA with few
-// query rows multiplies few zeros.  K and V go from memory to registers (every element belongs to one lane) and are split there; the order of dimensions and
-// positions within a product is chosen so that a lane's elements are 16 consecutive bytes.  HD: head_dim rounded up; ROWS: query rows in eights.
-template <int HD, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_constant__ PrefixParams p) {
-    extern __shared__ __align__(16) float sm[];
-    constexpr int kPitch = HD + 16;  // floats: lanes of two rows meet in different banks
+// query rows multiplies few zeros.  K and V of a tile come to the warp's own shared memory by tiled bulk copies: the next tile's K is asked for when this one's scores are there, its V
+// when its output is.  (Loaded into registers they take as much of L1 while they are on their way, and beside prefix_tc_kernel there is none: 114 us where this takes
+// LATER.)  They are split where they are used; which position and which dimensions a lane has is chosen so that its loads are 16 bytes and meet no others' banks.
+// HD: head_dim rounded up, or head_dim itself (EXACT); ROWS: query rows in eights.
+template <int HD, int ROWS, bool EXACT>
+__global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PartMaps maps) {
+    extern __shared__ __align__(1024) unsigned char smem[];
+    constexpr int kPitch = HD + 16;  // floats of a query row: lanes of two rows meet in different banks
     constexpr int kRows = ROWS * 8;
+    constexpr uint32_t kHalf = kKeys * HD * 4;  // K or V of a tile: per 32 dimensions 16 rows of 128 bytes, whose 16-byte pieces are exchanged by the row's number
+    __shared__ uint64_t bars[kWarps][2];
+    __shared__ int gave_up;
+    float *sm = reinterpret_cast<float *>(smem + kWarps * 2 * kHalf);
     uint32_t *q_hi = reinterpret_cast<uint32_t *>(sm), *q_lo = q_hi + kRows * kPitch;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t turned = (g >> 1) | ((g & 1u) << 2);  // g with its lowest bit as its highest: two neighbours are four rows, or pieces, apart
     yule_pdl_launch_dependents();
-    yule_pdl_wait();
+    // Behind the prefix on the tensor core nothing here depends on it, and what came before it is over (it waited, and let this kernel start): only one CTA's end waits, so that who
+    // waits for this kernel has waited for that one.
+    const bool waits = !p.beside || (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1);
+    if (!p.beside) yule_pdl_wait();
 
-    // which positions, for which rows
-    uint32_t item = blockIdx.x, kvh, row0, n_rows, key0, key1, slot;
-    const float *kc, *vc;
-    size_t stride;
-    if (item < p.prefix_items) {
-        slot = item % p.prefix_splits;
-        item /= p.prefix_splits;
-        kvh = item % p.n_kv_heads;
-        row0 = item / p.n_kv_heads * kRows;
+    // which positions, for which rows: x the rows (of the prefix's first), y the KV head, z the chunk
+    const uint32_t kvh = blockIdx.y, split = blockIdx.z;
+    uint32_t row0, n_rows, key0, key1, slot = split, line = 0;
+    const bool of_prefix = blockIdx.x < p.prefix_items;
+    if (of_prefix) {
+        row0 = blockIdx.x * kRows;
         n_rows = p.n_seqs * p.n_query * p.group;
-        key0 = slot * p.prefix_chunk;
-        key1 = min(key0 + p.prefix_chunk, p.prefix_len);
-        kc = p.prefix_k, vc = p.prefix_v, stride = p.prefix_stride;
+        key0 = split * p.prefix_chunk;
+        key1 = split < p.prefix_splits ? min(key0 + p.prefix_chunk, p.prefix_len) : key0;
     } else {
-        item -= p.prefix_items;
-        const uint32_t split = item % p.tail_splits;
-        item /= p.tail_splits;
-        kvh = item % p.n_kv_heads;
-        item /= p.n_kv_heads;
-        const uint32_t b = item / p.tail_row_tiles, first = b * p.n_query * p.group;
-        row0 = first + item % p.tail_row_tiles * kRows;
+        const uint32_t i = blockIdx.x - p.prefix_items, b = p.tail_row_tiles == 1 ? i : i / p.tail_row_tiles, first = b * p.n_query * p.group;
+        row0 = first + (i - b * p.tail_row_tiles) * kRows;
         n_rows = first + p.n_query * p.group;
         key0 = split * p.tail_chunk;
         const uint32_t seen = common_len(p, b);
-        if (key0 >= seen) return;
-        key1 = min(key0 + p.tail_chunk, seen);
-        slot = p.prefix_splits + split;
-        kc = p.tail_k + (size_t)b * p.tail_capacity * p.tail_stride, vc = p.tail_v + (size_t)b * p.tail_capacity * p.tail_stride, stride = p.tail_stride;
+        key1 = split < p.tail_splits && key0 < seen ? min(key0 + p.tail_chunk, seen) : key0;
+        slot += p.prefix_splits;
+        line = b * p.tail_capacity;  // the sequence's first row
     }
-    kc += (size_t)kvh * p.hd, vc += (size_t)kvh * p.hd;
-
+    if (key0 >= key1) {
+        if (waits) yule_pdl_wait();
+        return;
+    }
+    const uint32_t ring = smem_u32(smem) + warp * 2 * kHalf, bar = smem_u32(&bars[warp][0]);
+    const unsigned char *mine = smem + warp * 2 * kHalf;
+    auto copy = [&](uint32_t base, uint32_t which) {  // by one lane: K (0) or V of the tile
+        const uint64_t map = reinterpret_cast<uint64_t>(&maps.m[(of_prefix ? 0 : 2) + which]);
+        mbar_arrive_expect_tx(bar + 8 * which, kHalf);
+#pragma unroll
+        for (uint32_t i = 0; i < HD / 32; i++)  // (elements of eight bytes)
+            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(ring + which * kHalf + i * (kKeys * 128)), "l"(map),
+                         "r"(bar + 8 * which), "r"(kvh * (p.hd / 2) + 16 * i), "r"(line + base)
+                         : "memory");
+    };
+    const uint32_t first = key0 + warp * kKeys;
+    if (lane == 0) {
+        mbar_init(bar, 1);
+        mbar_init(bar + 8, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+        if (tid == 0) gave_up = 0;
+        if (first < key1) copy(first, 0), copy(first, 1);
+    }
     // query rows, in units of ln 2, as two terms
     for (uint32_t i = tid; i < kRows * (HD / 4); i += kWarps * 32) {
         const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4, row = row0 + r;
@@ -89,7 +118,7 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
     }
     __syncthreads();
 
-    // Per lane the rows 8n + 2t, 8n + 2t + 1, and of them the dimensions 32i + 4g .. 32i + 4g + 3.
+    // Per lane the rows 8n + 2t, 8n + 2t + 1, and of them the dimensions 32i + 4·turned on.
     float o[ROWS][HD / 32][2][4], m[ROWS][2], l[ROWS][2];
 #pragma unroll
     for (int n = 0; n < ROWS; n++) {
@@ -99,15 +128,30 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
 #pragma unroll
             for (int e = 0; e < 4; e++) o[n][i][0][e] = o[n][i][1][e] = 0.f;
     }
-    for (uint32_t base = key0 + warp * kKeys; base < key1; base += kTileKeys) {
-        const bool in0 = base + g < key1, in1 = base + g + 8 < key1;
-        const float *k0 = kc + (size_t)(base + g) * stride + 4 * t, *k1 = k0 + 8 * stride;
-        // Scores.  The tensor core truncates what it adds to, so the large products of four steps at a time have sums of their own.
-        float s[ROWS][4], small[ROWS][4];
+    uint32_t phase = 0;
+    bool ok = true;
+    auto await = [&](uint32_t which) {
+        ok = mbar_wait(bar + 8 * which, phase, &gave_up, p.status);
+        ok = __all_sync(0xffffffffu, ok);
+        return ok;
+    };
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t base = first; base < key1; base += kTileKeys, phase ^= 1u) {
+        const bool whole = base + kKeys <= key1;  // (what lies behind, in the tile or the row, may be anything)
+        const bool in0 = base + turned < key1, in1 = base + turned + 8 < key1;
+        // Scores of positions base + turned and base + turned + 8.  The tensor core truncates what it adds to, so the large products of four steps at a time have sums of their own.
+        // (With few query rows a sum of all small products would be a chain of as many steps as there are products: four sums.)
+        constexpr int kSums = ROWS == 1 ? 4 : 1;
+        float s[ROWS][4], small[ROWS][kSums][4];
 #pragma unroll
         for (int n = 0; n < ROWS; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[n][e] = small[n][e] = 0.f;
+            for (int e = 0; e < 4; e++) {
+                s[n][e] = 0.f;
+#pragma unroll
+                for (int c = 0; c < kSums; c++) small[n][c][e] = 0.f;
+            }
+        if (!await(0)) break;
 #pragma unroll
         for (int i = 0; i < HD / 32; i++) {
             float big[ROWS][4];
@@ -117,8 +161,9 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
                 for (int e = 0; e < 4; e++) big[n][e] = 0.f;
 #pragma unroll
             for (int j = 2 * i; j < 2 * i + 2; j++) {
-                const bool dims = 16 * j + 4 * t < p.hd;
-                const float4 a = load4(k0 + 16 * j, in0 && dims), b = load4(k1 + 16 * j, in1 && dims);
+                const unsigned char *at = mine + i * (kKeys * 128) + turned * 128 + ((((j & 1) * 4 + t) ^ turned) << 4);
+                float4 a = *reinterpret_cast<const float4 *>(at), b = *reinterpret_cast<const float4 *>(at + 8 * 128);
+                if (!EXACT && 16 * j + 4 * t >= p.hd) a = b = zero;
                 uint32_t ah[4], al[4], bh[4], bl[4];
                 split_tf32(a.x, ah[0], al[0]), split_tf32(a.y, ah[1], al[1]), split_tf32(a.z, ah[2], al[2]), split_tf32(a.w, ah[3], al[3]);
                 split_tf32(b.x, bh[0], bl[0]), split_tf32(b.y, bh[1], bl[1]), split_tf32(b.z, bh[2], bl[2]), split_tf32(b.w, bh[3], bl[3]);
@@ -126,11 +171,11 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
                 for (int n = 0; n < ROWS; n++) {
                     const uint4 qh = *reinterpret_cast<const uint4 *>(q_hi + (8 * n + g) * kPitch + 16 * j + 4 * t);
                     const uint4 ql = *reinterpret_cast<const uint4 *>(q_lo + (8 * n + g) * kPitch + 16 * j + 4 * t);
-                    mma_tf32(small[n], al[0], bl[0], al[1], bl[1], qh.x, qh.y);
-                    mma_tf32(small[n], ah[0], bh[0], ah[1], bh[1], ql.x, ql.y);
+                    mma_tf32(small[n][0], al[0], bl[0], al[1], bl[1], qh.x, qh.y);
+                    mma_tf32(small[n][1 % kSums], ah[0], bh[0], ah[1], bh[1], ql.x, ql.y);
                     mma_tf32(big[n], ah[0], bh[0], ah[1], bh[1], qh.x, qh.y);
-                    mma_tf32(small[n], al[2], bl[2], al[3], bl[3], qh.z, qh.w);
-                    mma_tf32(small[n], ah[2], bh[2], ah[3], bh[3], ql.z, ql.w);
+                    mma_tf32(small[n][2 % kSums], al[2], bl[2], al[3], bl[3], qh.z, qh.w);
+                    mma_tf32(small[n][3 % kSums], ah[2], bh[2], ah[3], bh[3], ql.z, ql.w);
                     mma_tf32(big[n], ah[2], bh[2], ah[3], bh[3], qh.z, qh.w);
                 }
             }
@@ -139,13 +184,19 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
 #pragma unroll
                 for (int e = 0; e < 4; e++) s[n][e] += big[n][e];
         }
-        // Soft-max: positions base + g (s[0], s[1]) and base + g + 8 (s[2], s[3]) of rows 8n + 2t and 8n + 2t + 1.
+        __syncwarp();
+        if (lane == 0 && base + kTileKeys < key1) copy(base + kTileKeys, 0);
+        // Soft-max of s[0], s[1] (the first position) and s[2], s[3] (the second) in rows 8n + 2t and 8n + 2t + 1.
         uint32_t ph[ROWS][4], pl[ROWS][4];
         float alpha[ROWS][2];
 #pragma unroll
         for (int n = 0; n < ROWS; n++) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[n][e] = (e < 2 ? in0 : in1) ? s[n][e] + small[n][e] : -INFINITY;
+            for (int e = 0; e < 4; e++) {
+                float rest = small[n][0][e];
+                if (kSums == 4) rest = (rest + small[n][1 % kSums][e]) + (small[n][2 % kSums][e] + small[n][3 % kSums][e]);
+                s[n][e] = (e < 2 ? in0 : in1) ? s[n][e] + rest : -INFINITY;
+            }
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 float mx = fmaxf(s[n][c], s[n][c + 2]);
@@ -160,16 +211,16 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
                 s[n][c + 2] = exp2f(s[n][c + 2] - from);
                 l[n][c] = fmaf(l[n][c], alpha[n][c], s[n][c] + s[n][c + 2]);
             }
-            // as the second operand of the output's products: row (position) t or t + 4 of each eight, column (query row) g
+            // as the second operand of the output's products: row (position) t or t + 4 of each eight, column (query row) g; position k of eight is the turned number of 2·(k % 4) + k / 4
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int key = (e & 1) * 4 + t, src = key * 4 + (int)(g >> 1), up = e >> 1;  // e: positions 0.., 4.., 8.., 12..
+                const int src = (2 * (int)t + (e & 1)) * 4 + (int)(g >> 1), up = e >> 1;  // e: positions t, t + 4, t + 8, t + 12
                 const float even = __shfl_sync(0xffffffffu, s[n][2 * up], src), odd = __shfl_sync(0xffffffffu, s[n][2 * up + 1], src);
                 split_tf32(g & 1 ? odd : even, ph[n][e], pl[n][e]);
             }
         }
-        // Output.  Position 8u + t and 8u + t + 4 of this lane, dimensions 32i + 4g on.
-        const float *v0 = vc + (size_t)(base + t) * stride + 4 * g;
+        // Output: positions t and t + 4 of each eight of this lane.
+        if (!await(1)) break;
 #pragma unroll
         for (int i = 0; i < HD / 32; i++) {
             float fresh[ROWS][2][4];
@@ -177,17 +228,22 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
             for (int n = 0; n < ROWS; n++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) fresh[n][0][e] = fresh[n][1][e] = 0.f;
-            const bool dims = 32 * i + 4 * g < p.hd;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const float4 a = load4(v0 + 32 * i + (size_t)(8 * u) * stride, dims && base + 8 * u + t < key1), b = load4(v0 + 32 * i + (size_t)(8 * u + 4) * stride, dims && base + 8 * u + t + 4 < key1);
+                const unsigned char *at = mine + kHalf + i * (kKeys * 128) + (8 * u + t) * 128;
+                float4 a = *reinterpret_cast<const float4 *>(at + ((turned ^ t) << 4)), b = *reinterpret_cast<const float4 *>(at + 4 * 128 + ((turned ^ (t + 4)) << 4));
+                if (!EXACT && 32 * i + 4 * turned >= p.hd) a = b = zero;
+                if (!whole) {
+                    if (base + 8 * u + t >= key1) a = zero;
+                    if (base + 8 * u + t + 4 >= key1) b = zero;
+                }
                 uint32_t ah[4], al[4], bh[4], bl[4];
                 split_tf32(a.x, ah[0], al[0]), split_tf32(a.y, ah[1], al[1]), split_tf32(a.z, ah[2], al[2]), split_tf32(a.w, ah[3], al[3]);
                 split_tf32(b.x, bh[0], bl[0]), split_tf32(b.y, bh[1], bl[1]), split_tf32(b.z, bh[2], bl[2]), split_tf32(b.w, bh[3], bl[3]);
 #pragma unroll
                 for (int n = 0; n < ROWS; n++)
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {  // dimensions 32i + 4g + 2c and the next one
+                    for (int c = 0; c < 2; c++) {  // dimensions 32i + 4·turned + 2c and the next one
                         mma_tf32(fresh[n][c], al[2 * c], al[2 * c + 1], bl[2 * c], bl[2 * c + 1], ph[n][2 * u], ph[n][2 * u + 1]);
                         mma_tf32(fresh[n][c], ah[2 * c], ah[2 * c + 1], bh[2 * c], bh[2 * c + 1], pl[n][2 * u], pl[n][2 * u + 1]);
                         mma_tf32(fresh[n][c], ah[2 * c], ah[2 * c + 1], bh[2 * c], bh[2 * c + 1], ph[n][2 * u], ph[n][2 * u + 1]);
@@ -199,6 +255,13 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
                 for (int c = 0; c < 2; c++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) o[n][i][c][e] = fmaf(o[n][i][c][e], alpha[n][e & 1], fresh[n][c][e]);
+        }
+        __syncwarp();
+        if (lane == 0 && base + kTileKeys < key1) copy(base + kTileKeys, 1);
+    }
+    if (!ok) {  // gave up: the copies that are on their way have a moment to arrive (the status word says that nothing here counts)
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {
         }
     }
 
@@ -217,7 +280,7 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
             if (g == 0) ml[2 * r] = m[n][c], ml[2 * r + 1] = sum;
 #pragma unroll
             for (int i = 0; i < HD / 32; i++)
-                *reinterpret_cast<float4 *>(part + r * HD + 32 * i + 4 * g) = make_float4(o[n][i][0][c], o[n][i][0][2 + c], o[n][i][1][c], o[n][i][1][2 + c]);
+                *reinterpret_cast<float4 *>(part + r * HD + 32 * i + 4 * turned) = make_float4(o[n][i][0][c], o[n][i][0][2 + c], o[n][i][1][c], o[n][i][1][2 + c]);
         }
     __syncthreads();
     for (uint32_t i = tid; i < kRows * (HD / 4); i += kWarps * 32) {
@@ -238,6 +301,7 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
         if (d == 0) p.part_ml[at] = make_float2(mx, sum);
         *reinterpret_cast<float4 *>(p.part_o + at * p.hd + d) = acc;
     }
+    if (waits) yule_pdl_wait();
 }
 
 // A warp per (token, head): the parts in the order of their slots, then the newest positions one by one.
@@ -253,22 +317,35 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const __grid_constant
     const float2 *ml = p.part_ml + (size_t)row * p.slots;
     const float *po = p.part_o + (size_t)row * p.slots * p.hd;
     float m = -INFINITY, l = 0.f;
-    for (uint32_t s = lane; s < slots; s += 32) m = fmaxf(m, __ldcg(&ml[s].x));
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     float4 o[N];
 #pragma unroll
     for (int i = 0; i < N; i++) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float from = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-    for (uint32_t s = 0; s < slots; s++) {
-        const float2 x = __ldcg(ml + s);
-        const float f = exp2f(x.x - from);
-        l = fmaf(f, x.y, l);
+    // the parts of sixteen slots at a time on their way (of eight with two vectors of four a lane), added in the order of the slots
+    constexpr int kParts = 16 / N;
+    for (uint32_t s0 = 0; s0 < slots; s0 += kParts) {
+        float4 v[kParts][N];
+        const float2 x = lane < kParts && s0 + lane < slots ? __ldcg(ml + s0 + lane) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float4 v = load4(po + (size_t)s * p.hd + 4 * (lane + 32 * i), 4 * (lane + 32 * i) < p.hd);
-            o[i].x = fmaf(f, v.x, o[i].x), o[i].y = fmaf(f, v.y, o[i].y), o[i].z = fmaf(f, v.z, o[i].z), o[i].w = fmaf(f, v.w, o[i].w);
+        for (int e = 0; e < kParts; e++)
+#pragma unroll
+            for (int i = 0; i < N; i++) v[e][i] = load4(po + (size_t)(s0 + e) * p.hd + 4 * (lane + 32 * i), s0 + e < slots && 4 * (lane + 32 * i) < p.hd);
+        float most = x.x;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        most = fmaxf(most, m);
+        const float from = most == -INFINITY ? 0.f : most, alpha = exp2f(m - from), f = exp2f(x.x - from);
+        m = most;
+        float sum = f * x.y;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        l = fmaf(l, alpha, sum);
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i].x *= alpha, o[i].y *= alpha, o[i].z *= alpha, o[i].w *= alpha;
+#pragma unroll
+        for (int e = 0; e < kParts; e++) {
+            const float w = __shfl_sync(0xffffffffu, f, e);
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i].x = fmaf(w, v[e][i].x, o[i].x), o[i].y = fmaf(w, v[e][i].y, o[i].y), o[i].z = fmaf(w, v[e][i].z, o[i].z), o[i].w = fmaf(w, v[e][i].w, o[i].w);
         }
     }
     if (common < seen) {
@@ -305,17 +382,21 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const __grid_constant
         if (4 * (lane + 32 * i) < p.hd) *reinterpret_cast<float4 *>(to + 4 * (lane + 32 * i)) = make_float4(o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv);
 }
 
-template <int HD, int ROWS>
-cudaError_t launch_part(const PrefixParams &p, uint32_t items, bool pdl, cudaStream_t s, uint64_t *launches) {
-    constexpr size_t query = (size_t)2 * ROWS * 8 * (HD + 16) * 4, meeting = (size_t)kWarps * ROWS * 8 * (HD + 2) * 4, smem = query > meeting ? query : meeting;
-    auto kern = prefix_part_kernel<HD, ROWS>;
-    if (smem > 48 * 1024) {
+template <int HD, int ROWS, bool EXACT>
+cudaError_t launch_part(const PrefixParams &p, const PartMaps &maps, dim3 items, bool pdl, cudaStream_t s) {
+    constexpr size_t query = (size_t)2 * ROWS * 8 * (HD + 16) * 4, meeting = (size_t)kWarps * ROWS * 8 * (HD + 2) * 4;
+    constexpr size_t smem = (size_t)kWarps * 2 * kKeys * HD * 4 + (query > meeting ? query : meeting);
+    auto kern = prefix_part_kernel<HD, ROWS, EXACT>;
+    if (smem > 47 * 1024) {  // (beside a kilobyte of its own)
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // (of the current device)
         if (e != cudaSuccess) return e;
     }
-    const cudaError_t e = launch_kernel(kern, dim3(items), dim3(kWarps * 32), smem, s, pdl, p);
-    if (e == cudaSuccess) ++*launches;
-    return e;
+    return launch_kernel(kern, items, dim3(kWarps * 32), smem, s, pdl, p, maps);
+}
+template <int HD>
+cudaError_t launch_rows(const PrefixParams &p, const PartMaps &maps, uint32_t rows, dim3 items, bool pdl, cudaStream_t s) {
+    if (p.hd == HD) return rows == 1 ? launch_part<HD, 1, true>(p, maps, items, pdl, s) : rows == 2 ? launch_part<HD, 2, true>(p, maps, items, pdl, s) : launch_part<HD, 3, true>(p, maps, items, pdl, s);
+    return rows == 1 ? launch_part<HD, 1, false>(p, maps, items, pdl, s) : rows == 2 ? launch_part<HD, 2, false>(p, maps, items, pdl, s) : launch_part<HD, 3, false>(p, maps, items, pdl, s);
 }
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
@@ -330,10 +411,11 @@ Cut shape_of(const PrefixAttention &a, int sm_count, PrefixParams *p) {
     Cut cut;
     cut.tc = prefix_tc_supported(a.hd) && all >= 32 && a.prefix_len >= 64;
     if (const char *e = knob("YULE_PREFIX_TC")) cut.tc = prefix_tc_supported(a.hd) && atoi(e) != 0 && a.prefix_len > 0;
-    cut.rows = mine > 8 && a.hd <= 128 ? 2 : 1;
+    cut.rows = a.hd > 128 || mine <= 8 ? 1 : mine <= 16 ? 2 : 3;
     p->group = group;
     // Chunks such that the CTAs are a few per SM, of at least one tile for every warp.
-    const uint32_t want = 4 * sm_count;
+    uint32_t want = 8 * sm_count;
+    if (const char *e = knob("YULE_PREFIX_WANT")) want = atoi(e) * sm_count;
     auto chunk = [&](uint64_t units, uint32_t len) {
         const uint64_t per = units ? (want + units - 1) / units : 1;
         const uint64_t c = ((len + per - 1) / per + kTileKeys - 1) / kTileKeys * kTileKeys;
@@ -345,7 +427,7 @@ Cut shape_of(const PrefixAttention &a, int sm_count, PrefixParams *p) {
         const uint64_t units = (uint64_t)a.n_kv_heads * p->prefix_row_tiles;
         const uint32_t tiles = ceil_div(a.prefix_len, kPrefixTcKeys);
         double least = 1e30;
-        for (uint32_t s = 1; s <= tiles && s <= 64; s++) {
+        for (uint32_t s = ceil_div(tiles, kPrefixTcTiles), most = s + 63; s <= tiles && s <= most; s++) {
             const uint32_t each = ceil_div(tiles, s);
             const double rounds = (double)((units * ceil_div(tiles, each) + sm_count - 1) / sm_count), cost = rounds * (4.0 + each) + 0.05 * s;
             if (cost < least) least = cost, p->prefix_chunk = each * kPrefixTcKeys;
@@ -363,13 +445,18 @@ Cut shape_of(const PrefixAttention &a, int sm_count, PrefixParams *p) {
     return cut;
 }
 
+size_t parts_bytes(const PrefixAttention &a, const PrefixParams &p) {
+    const size_t parts = (size_t)a.n_seqs * a.n_query * a.n_heads * p.slots;
+    return (parts * (sizeof(float2) + (size_t)a.hd * sizeof(float)) + 127) / 128 * 128;
+}
+
 }  // namespace
 
 size_t prefix_attention_scratch_bytes(const PrefixAttention &a, int sm_count) {
     PrefixParams p = {};
-    shape_of(a, sm_count, &p);
-    const size_t parts = (size_t)a.n_seqs * a.n_query * a.n_heads * p.slots;
-    return parts * (sizeof(float2) + (size_t)a.hd * sizeof(float)) + 256;
+    const Cut cut = shape_of(a, sm_count, &p);
+    p.prefix_len = a.prefix_len, p.n_kv_heads = a.n_kv_heads, p.hd = a.hd;
+    return parts_bytes(a, p) + (cut.tc ? prefix_tc_scratch_bytes(p) : 0);
 }
 
 cudaError_t launch_prefix_attention(const PrefixAttention &a, int sm_count, cudaStream_t s, uint64_t *launches) {
@@ -384,23 +471,36 @@ cudaError_t launch_prefix_attention(const PrefixAttention &a, int sm_count, cuda
     p.part_ml = reinterpret_cast<float2 *>(p.part_o + parts * a.hd);
     p.status = a.status;
     const uint64_t out_rows = (uint64_t)a.n_seqs * a.n_query * a.n_heads;
-    uint64_t items = (uint64_t)a.n_seqs * p.n_kv_heads * p.tail_row_tiles * p.tail_splits;
-    if (!cut.tc) items += (uint64_t)p.n_kv_heads * p.prefix_row_tiles * p.prefix_splits;
-    if (items > 0x7FFFFFFFu || out_rows > 0x7FFFFFFFu) return cudaErrorInvalidValue;
+    p.beside = cut.tc;
+    p.prefix_items = cut.tc ? 0 : p.prefix_splits ? p.prefix_row_tiles : 0;
+    const uint64_t items = p.prefix_items + (p.tail_splits ? (uint64_t)a.n_seqs * p.tail_row_tiles : 0);
+    const uint32_t splits = !cut.tc && p.prefix_splits > p.tail_splits ? p.prefix_splits : p.tail_splits;
+    if (items > 0x7FFFFFFFu || out_rows > 0x7FFFFFFFu || a.n_kv_heads > 65535 || splits > 65535) return cudaErrorInvalidValue;
     cudaError_t e = cudaSuccess;
     bool pdl = a.pdl;
     if (cut.tc) {
-        if ((e = launch_prefix_tc(p, pdl, s, launches)) != cudaSuccess) return e;
+        if ((e = launch_prefix_tc(p, static_cast<unsigned char *>(a.scratch) + parts_bytes(a, p), pdl, s, launches)) != cudaSuccess) return e;
         pdl = true;
     }
-    p.prefix_items = cut.tc ? 0 : p.n_kv_heads * p.prefix_row_tiles * p.prefix_splits;
     if (items) {
-#define YULE_PART(H) e = cut.rows == 1 ? launch_part<H, 1>(p, (uint32_t)items, pdl, s, launches) : launch_part<H, 2>(p, (uint32_t)items, pdl, s, launches)
-        if (a.hd <= 64) YULE_PART(64);
-        else if (a.hd <= 96) YULE_PART(96);
-        else if (a.hd <= 128) YULE_PART(128);
-        else e = launch_part<256, 1>(p, (uint32_t)items, pdl, s, launches);
-#undef YULE_PART
+        alignas(64) PartMaps maps = {};
+        auto map = [&](const float *at, uint64_t rows, size_t stride, CUtensorMap *to) {
+            return cached_tensor_map_2d(at, 8, (uint64_t)a.n_kv_heads * a.hd / 2, rows, stride * 4, 16, kKeys, to, 128);
+        };
+        if (p.prefix_items) {
+            e = map(a.prefix_k, a.prefix_len, p.prefix_stride, &maps.m[0]);
+            if (e == cudaSuccess) e = map(a.prefix_v, a.prefix_len, p.prefix_stride, &maps.m[1]);
+        }
+        if (p.tail_splits && e == cudaSuccess) {
+            const uint64_t rows = (uint64_t)a.n_seqs * a.tail_capacity;
+            e = map(a.tail_k, rows, p.tail_stride, &maps.m[2]);
+            if (e == cudaSuccess) e = map(a.tail_v, rows, p.tail_stride, &maps.m[3]);
+        }
+        if (e != cudaSuccess) return e;
+        const dim3 n((uint32_t)items, a.n_kv_heads, splits);
+        e = a.hd <= 64 ? launch_rows<64>(p, maps, cut.rows, n, pdl, s) : a.hd <= 96 ? launch_rows<96>(p, maps, cut.rows, n, pdl, s) : a.hd <= 128 ? launch_rows<128>(p, maps, cut.rows, n, pdl, s)
+                                                                                                      : launch_part<256, 1, false>(p, maps, n, pdl, s);
+        ++*launches;
         if (e != cudaSuccess) return e;
         pdl = true;
     }
