@@ -1,5 +1,6 @@
 """The hand-offs of the shared prefix on tcgen05 (csrc/prefix_attention_tc.cu) under random interleavings, on the CPU: three buffers of K, two of V, of scores and of
-probabilities by tile parity, waits that know a phase's parity only, MMAs and copies that run in the order of their issue some time after it, and the words through which the halves of a row meet."""
+probabilities by tile parity, waits that know a phase's parity only, MMAs and copies that run in the order of their issue
+(scores and outputs each in theirs) some time after it, and the words through which the halves of a row meet."""
 
 import random
 
@@ -7,7 +8,7 @@ import pytest
 
 from interleavings import Barrier, interleave
 
-SOFT, SUM = 8, 4
+SOFT, SUM, PARTS = 8, 4, 2
 
 
 class Meeting:
@@ -29,13 +30,13 @@ def simulate(seed, n, k_wait=True, v_wait=True, alpha_wait=True, s_wait=True, o_
     pair = lambda c: [Barrier(c), Barrier(c)]  # noqa: E731
     k_full, k_empty = [Barrier(1) for _ in range(3)], [Barrier(1) for _ in range(3)]
     v_full, v_empty, s_full, s_empty, p_full, a_empty = pair(1), pair(1), pair(1), pair(SOFT), pair(SOFT), pair(SUM)
-    o_full, o_empty, l_full = Barrier(2), Barrier(SUM), Barrier(SOFT)
+    o_full, o_empty, l_full = pair(2), pair(SUM), Barrier(SOFT)
     meet_rows = [Meeting(2) for _ in range(4)]
-    K, V, S, P, O = [None] * 3, [None] * 2, [None] * 2, [[None] * SOFT for _ in range(2)], None
+    K, V, S, P, O = [None] * 3, [None] * 2, [None] * 2, [[None] * SOFT for _ in range(2)], [None] * PARTS
     alpha = [[None] * SUM for _ in range(2)]
-    k_used, v_used, p_used, s_read, o_read, alpha_read = {-1, -2, -3}, {-1, -2}, {-1, -2}, [[-2 + b] * SOFT for b in range(2)], [-1] * SUM, [[-2 + b] * SUM for b in range(2)]
+    k_used, v_used, p_used, s_read, o_read, alpha_read = {-1, -2, -3}, {-1, -2}, {-1, -2}, [[-2 + b] * SOFT for b in range(2)], [[-1] * SUM for _ in range(PARTS)], [[-2 + b] * SUM for b in range(2)]
     rows, rows_read = [[[None] * 2 for _ in range(2)] for _ in range(4)], [[-1] * 2 for _ in range(4)]
-    queue, copies = [], []
+    queue, outputs, copies = [], [], []
 
     def loader():
         def copy(to, used, j):
@@ -84,7 +85,7 @@ def simulate(seed, n, k_wait=True, v_wait=True, alpha_wait=True, s_wait=True, o_
             p_full[b].arrive()
         l_full.arrive()
 
-    def issue():
+    def issue_scores():
         def scores(j):
             def go():
                 b = j & 1
@@ -94,46 +95,52 @@ def simulate(seed, n, k_wait=True, v_wait=True, alpha_wait=True, s_wait=True, o_
                 k_used.add(j)
             return go
 
-        def output(j):
+        for j in range(n):
+            if s_wait:
+                yield lambda: s_empty[j & 1].over(j >> 1 & 1 ^ 1)
+            yield lambda: k_full[j % 3].over(j // 3 & 1)
+            queue.extend([scores(j), k_empty[j % 3].arrive, s_full[j & 1].arrive])
+
+    def issue_output():
+        def output(j, part):
             def go():
-                nonlocal O
                 assert V[j & 1] == j and P[j & 1] == [j] * SOFT, "output of other operands"
-                assert o_read == [j - 1] * SUM, "output overwritten before it was read"
-                O = j
-                v_used.add(j)
-                p_used.add(j)
+                assert o_read[part] == [j - 1] * SUM, "output overwritten before it was read"
+                O[part] = j
+                if part + 1 == PARTS:
+                    v_used.add(j)
+                    p_used.add(j)
             return go
 
-        for j in range(-2, n):
-            if j + 2 < n:
-                i = j + 2
-                if s_wait:
-                    yield lambda: s_empty[i & 1].over(i >> 1 & 1 ^ 1)
-                yield lambda: k_full[i % 3].over(i // 3 & 1)
-                queue.extend([scores(i), k_empty[i % 3].arrive, s_full[i & 1].arrive])
-            if j >= 0:
-                b, ph = j & 1, j >> 1 & 1
-                yield lambda: v_full[b].over(ph)
+        for j in range(n):
+            b, ph = j & 1, j >> 1 & 1
+            yield lambda: v_full[b].over(ph)
+            yield lambda: p_full[b].over(ph)
+            for part in range(PARTS):
                 if o_wait:
-                    yield lambda: o_empty.over(j & 1 ^ 1)
-                yield lambda: p_full[b].over(ph)
-                queue.extend([output(j), v_empty[b].arrive, o_full.arrive])
-                o_full.arrive()
+                    yield lambda: o_empty[part].over(j & 1 ^ 1)
+                outputs.append(output(j, part))
+                if part + 1 == PARTS:
+                    outputs.append(v_empty[b].arrive)
+                outputs.append(o_full[part].arrive)
+                o_full[part].arrive()
 
     def sums(w):
         for j in range(n):
-            yield lambda: o_full.over(j & 1)
-            assert O == j and alpha[j & 1][w] == j, "output or alpha of another tile"
-            alpha_read[j & 1][w] = j
-            a_empty[j & 1].arrive()
-            yield lambda: True
-            assert O == j
-            o_read[w] = j
-            o_empty.arrive()
+            for part in range(PARTS):
+                yield lambda: o_full[part].over(j & 1)
+                assert O[part] == j and alpha[j & 1][w] == j, "output or alpha of another tile"
+                if part + 1 == PARTS:
+                    alpha_read[j & 1][w] = j
+                    a_empty[j & 1].arrive()
+                yield lambda: True
+                assert O[part] == j
+                o_read[part][w] = j
+                o_empty[part].arrive()
         yield lambda: l_full.over(0)
-        assert k_used >= set(range(n)) and v_used >= set(range(n)) and not queue and not copies, "the operands' memory taken while they are in use"
+        assert k_used >= set(range(n)) and v_used >= set(range(n)) and not queue and not outputs and not copies, "the operands' memory taken while they are in use"
 
-    interleave(rng, [issue(), loader()] + [softmax(w) for w in range(SOFT)] + [sums(w) for w in range(SUM)], [queue, copies])
+    interleave(rng, [issue_scores(), issue_output(), loader()] + [softmax(w) for w in range(SOFT)] + [sums(w) for w in range(SUM)], [queue, outputs, copies])
 
 
 @pytest.mark.parametrize("n", [1, 2, 3, 4, 9, 14])

@@ -9,8 +9,9 @@
 // then hi·hi; outputs of tiles are added up in fp32, with the mean of what truncation takes given back.  A value that is not finite makes every row's output not
 // finite: every row sees it.
 //
-// Roles (512 threads): eight warps do the soft-max (a thread per row and half a tile's positions), four add the output up (a thread per row), one issues the MMAs, one the bulk
-// copies.  The query rows are in tensor memory; K has three buffers, V, scores and probabilities have two, and the scores of a tile are issued two tiles ahead of its output.  (Converting K and V where they are used took 5000 to 7400 clocks a tile and CTA, by
+// Roles (512 threads): eight warps do the soft-max (a thread per row and half a tile's positions), four add the output up (a thread per row), two issue the MMAs of scores and of
+// output (one that does both waits for either 2900 clocks a tile), one the bulk copies.  The query rows are in tensor memory; K has three buffers, V, scores and probabilities have two, and the scores of a tile are issued two tiles ahead of its output,
+// which comes in parts of 64 dimensions: one is added up while the next is multiplied.  (Converting K and V where they are used took 5000 to 7400 clocks a tile and CTA, by
 // the soft-max warps or by eight more: the MMAs take 1536.)
 
 #include <cfloat>
@@ -29,7 +30,7 @@ namespace {
 constexpr int kRows = (int)kPrefixTcRows;  // query rows per CTA = TMEM lanes
 constexpr int kKeys = (int)kPrefixTcKeys;  // positions per tile
 constexpr int kThreads = 512;
-constexpr uint32_t kSumWarp = 8, kMmaWarp = 12, kLoadWarp = 13;  // the first of each; soft-max from 0 on
+constexpr uint32_t kSumWarp = 8, kMmaWarp = 12, kLoadWarp = 13, kOutputWarp = 14;  // the first of each; soft-max from 0 on
 constexpr int kLaunchRegs = 96;  // registers per thread that 512 threads are launched with (the build checks that the kernels get them)
 constexpr int kSoftRegs = 96, kSumRegs = 168, kIssueRegs = 24;
 static_assert(2 * kSoftRegs + kSumRegs + kIssueRegs <= 4 * kLaunchRegs, "register split");
@@ -68,7 +69,7 @@ struct Layout {
     static constexpr uint32_t kOffK = 0, kOffV = 6 * kPlane, kOffRows = 10 * kPlane;  // three buffers of K, two of V
     // per row: alpha (two tiles), largest score of either half (two tiles), sums of either half, last largest score, score factor; then inverse scales of K and V of the chunk's
     // tiles; then barriers
-    static constexpr uint32_t kOffScales = kOffRows + 10 * kRows * 4, kOffBars = kOffScales + kMostTiles * 8, kBars = 22;
+    static constexpr uint32_t kOffScales = kOffRows + 10 * kRows * 4, kOffBars = kOffScales + kMostTiles * 8, kBars = 24;
     static constexpr uint32_t kSmem = kOffBars + kBars * 8 + 16;
     // before the first tile the query rows as packed words (where the last K and V will be), behind the last one the output, a row after the other
     static constexpr uint32_t kPitch = HD + 4, kOffQ = 4 * kPlane;
@@ -147,7 +148,8 @@ __global__ void __launch_bounds__(640, 1) prefix_tc_kernel(  // (so many threads
     const __grid_constant__ PrefixParams p, const unsigned char *tiles, const float2 *scales, uint32_t slot0, uint32_t tiles_in_memory) {
     using L = Layout<HD>;
     extern __shared__ __align__(128) unsigned char smem[];
-    constexpr int KS = HD / 16;  // k16 steps of a score
+    constexpr int KS = HD / 16;           // k16 steps of a score
+    constexpr uint32_t kParts = HD / 64;  // of the output
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t slot = slot0 + blockIdx.x, row0 = blockIdx.y * kRows, kvh = blockIdx.z, n_rows = p.n_seqs * p.n_query * p.group;
     const uint32_t key0 = slot * p.prefix_chunk, keys = min(p.prefix_chunk, p.prefix_len - key0), n_tiles = (keys + kKeys - 1) / kKeys;
@@ -158,9 +160,9 @@ __global__ void __launch_bounds__(640, 1) prefix_tc_kernel(  // (so many threads
     float2 *inverse = reinterpret_cast<float2 *>(smem + L::kOffScales);  // of K and V, by tile
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kOffBars);
     const uint32_t bar0 = smem_u32(bars);
-    // pairs by tile parity: V there, free (and the probabilities used); scores there, free; probabilities there; alpha free; three: K there, free; else one: output there, free; sums there
+    // pairs by tile parity: V there, free (and the probabilities used); scores there, free; probabilities there; alpha free; three: K there, free; by part: output there, free; else one: sums there
     const uint32_t v_full = bar0, v_empty = bar0 + 16, s_full = bar0 + 32, s_empty = bar0 + 48, p_full = bar0 + 64, a_empty = bar0 + 80, k_full = bar0 + 96, k_empty = bar0 + 120,
-                   o_full = bar0 + 144, o_empty = bar0 + 152, l_full = bar0 + 160;
+                   o_full = bar0 + 144, o_empty = bar0 + 160, l_full = bar0 + 176;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     if (tid == 0) {
@@ -175,9 +177,9 @@ __global__ void __launch_bounds__(640, 1) prefix_tc_kernel(  // (so many threads
             mbar_init(s_empty + 8 * b, 8);
             mbar_init(p_full + 8 * b, 8);
             mbar_init(a_empty + 8 * b, 4);
+            mbar_init(o_full + 8 * b, 2);  // tcgen05.commit, and the thread that saw the probabilities (and with them alpha) arrive
+            mbar_init(o_empty + 8 * b, 4);
         }
-        mbar_init(o_full, 2);  // tcgen05.commit, and the thread that saw the probabilities (and with them alpha) arrive
-        mbar_init(o_empty, 4);
         mbar_init(l_full, 8);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -246,71 +248,72 @@ __global__ void __launch_bounds__(640, 1) prefix_tc_kernel(  // (so many threads
     tc_fence_after();
     if (warp >= kMmaWarp) {
         move_registers<true, kIssueRegs, kLaunchRegs>();
+        constexpr uint32_t idesc = (1u << 4) | (64u >> 3 << 17) | ((uint32_t)(kRows >> 4) << 24);  // fp16 × fp16 → fp32, K-major, M = 128, N = 64 positions, or dimensions of a part
+        constexpr uint64_t plane = L::kPlane >> 4;
+        static_assert(kKeys == 64, "N");
+        bool ok = true;
+        auto await = [&](uint32_t bar, uint32_t parity) {
+            ok = ok && mbar_wait(bar, parity, abort_flag, p.status);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+            return ok;
+        };
+        const uint32_t base = smem_u32(smem);
         if (warp == kMmaWarp) {
-            constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);  // fp16 × fp16 → fp32, K-major, M = 128, N = 64
-            constexpr uint32_t idesc_o = (1u << 4) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);     // N = head_dim
-            constexpr uint64_t plane = L::kPlane >> 4;
-            bool ok = true;
-            auto await = [&](uint32_t bar, uint32_t parity) {
-                ok = ok && mbar_wait(bar, parity, abort_flag, p.status);
-                ok = __all_sync(0xffffffffu, ok);
-                tc_fence_after();
-                return ok;
-            };
-            const uint32_t base = smem_u32(smem);
-            RingPos kr;  // of the next tile's K
-            auto scores = [&](uint32_t j) {
+            RingPos kr;
+            for (uint32_t j = 0; j < n_tiles; j++, kr.advance(3)) {
                 const uint32_t b = j & 1u;
-                if (!await(s_empty + 8 * b, ((j >> 1) & 1u) ^ 1u) || !await(k_full + 8 * kr.s, kr.ph)) return;
+                if (!await(k_full + 8 * kr.s, kr.ph) || !await(s_empty + 8 * b, ((j >> 1) & 1u) ^ 1u)) break;
                 const uint32_t d = tmem_base + L::kS + b * 64, q_hi = tmem_base + L::kQ, q_lo = q_hi + HD / 2;
                 const uint64_t kd = smem_desc(base + L::kOffK + kr.s * 2 * L::kPlane, kKeys * 16, 128);
                 constexpr uint64_t step = (2 * kKeys * 16) >> 4;
                 if (elect_one()) {
                     mma_steps<0, KS>([&](auto ic) {
                         constexpr uint32_t i = decltype(ic)::value;
-                        umma_f16_ts<(i != 0)>(d, q_lo + 8 * i, kd + i * step, idesc_s);
-                        umma_f16_ts<1>(d, q_hi + 8 * i, kd + i * step + plane, idesc_s);
+                        umma_f16_ts<(i != 0)>(d, q_lo + 8 * i, kd + i * step, idesc);
+                        umma_f16_ts<1>(d, q_hi + 8 * i, kd + i * step + plane, idesc);
                     });
                     mma_steps<0, KS>([&](auto ic) {
                         constexpr uint32_t i = decltype(ic)::value;
-                        umma_f16_ts<1>(d, q_hi + 8 * i, kd + i * step, idesc_s);
+                        umma_f16_ts<1>(d, q_hi + 8 * i, kd + i * step, idesc);
                     });
                     umma_commit(k_empty + 8 * kr.s);
                     umma_commit(s_full + 8 * b);
                 }
                 __syncwarp();
-                kr.advance(3);
-            };
-            scores(0);
-            if (n_tiles > 1) scores(1);
+            }
+        } else if (warp == kOutputWarp) {
             for (uint32_t j = 0; j < n_tiles && ok; j++) {
-                if (j + 2 < n_tiles) scores(j + 2);  // (as soon as this tile's scores have been read: under its soft-max)
-                if (!ok) break;
                 const uint32_t b = j & 1u, ph = (j >> 1) & 1u;
-                if (!await(v_full + 8 * b, ph) || !await(o_empty, (j & 1u) ^ 1u) || !await(p_full + 8 * b, ph)) break;
+                if (!await(v_full + 8 * b, ph) || !await(p_full + 8 * b, ph)) break;
                 const uint64_t vd = smem_desc(base + L::kOffV + b * 2 * L::kPlane, HD * 16, 128);
                 constexpr uint64_t step = (2 * HD * 16) >> 4;
-                const uint32_t d = tmem_base + L::kO, hi = tmem_base + L::kP + b * 64, lo = hi + 32;
-                if (elect_one()) {
-                    mma_steps<0, 4>([&](auto ic) {
-                        constexpr uint32_t i = decltype(ic)::value;
-                        umma_f16_ts<(i != 0)>(d, lo + 8 * i, vd + i * step, idesc_o);
-                        umma_f16_ts<1>(d, hi + 8 * i, vd + i * step + plane, idesc_o);
-                    });
-                    mma_steps<0, 4>([&](auto ic) {
-                        constexpr uint32_t i = decltype(ic)::value;
-                        umma_f16_ts<1>(d, hi + 8 * i, vd + i * step, idesc_o);
-                    });
-                    umma_commit(v_empty + 8 * b);
-                    umma_commit(o_full);  // (the last of all: what waits for the last tile's knows that nothing is under way)
-                    mbar_arrive(o_full);
-                }
-                __syncwarp();
+                const uint32_t hi = tmem_base + L::kP + b * 64, lo = hi + 32;
+                mma_steps<0, kParts>([&](auto pc) {
+                    constexpr uint32_t part = decltype(pc)::value;
+                    constexpr uint64_t dims = (part * 64 * 16) >> 4;
+                    if (!ok || !await(o_empty + 8 * part, (j & 1u) ^ 1u)) return;
+                    const uint32_t d = tmem_base + L::kO + 64 * part;
+                    if (elect_one()) {
+                        mma_steps<0, 4>([&](auto ic) {
+                            constexpr uint32_t i = decltype(ic)::value;
+                            umma_f16_ts<(i != 0)>(d, lo + 8 * i, vd + i * step + dims, idesc);
+                            umma_f16_ts<1>(d, hi + 8 * i, vd + i * step + dims + plane, idesc);
+                        });
+                        mma_steps<0, 4>([&](auto ic) {
+                            constexpr uint32_t i = decltype(ic)::value;
+                            umma_f16_ts<1>(d, hi + 8 * i, vd + i * step + dims, idesc);
+                        });
+                        if (part + 1 == kParts) umma_commit(v_empty + 8 * b);
+                        umma_commit(o_full + 8 * part);  // (the last of all: what waits for the last tile's knows that nothing is under way)
+                        mbar_arrive(o_full + 8 * part);
+                    }
+                    __syncwarp();
+                });
             }
         } else if (warp == kLoadWarp && lane == 0) {
             RingPos kr;
             kr.advance(3), kr.advance(3);
-            bool ok = true;
             for (uint32_t j = 0; j < n_tiles && ok; j++) {  // V of this tile, K of the one after the next
                 const uint32_t b = j & 1u;
                 ok = mbar_wait(v_empty + 8 * b, ((j >> 1) & 1u) ^ 1u, abort_flag, p.status);
@@ -398,61 +401,73 @@ __global__ void __launch_bounds__(640, 1) prefix_tc_kernel(  // (so many threads
 #pragma unroll
         for (int i = 0; i < HD / 2; i++) o[i] = 0;
         bool ok = true;
-        for (uint32_t j = 0; j < n_tiles; j++) {
-            ok = mbar_wait(o_full, j & 1u, abort_flag, p.status);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
-            const float alpha = alpha_row[(j & 1u) * kRows + r], vi = inverse[j].y;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(a_empty + 8 * (j & 1u));
-            const uint64_t alpha2 = pair(alpha, alpha), vi2 = pair(vi, vi);
+        for (uint32_t j = 0; j < n_tiles && ok; j++) {
+            float alpha = 0.f;
+            const float vi = inverse[j].y;
 #pragma unroll
-            for (uint32_t c0 = 0; c0 < HD; c0 += 16) {
-                uint32_t y[16];
-                tmem_ld16_issue(tmem_base + lanes + L::kO + c0, y);
-                tmem_ld_wait();
-                if (c0 + 16 == HD) {
-                    tc_fence_before();
+            for (uint32_t part = 0; part < kParts; part++) {
+                ok = ok && mbar_wait(o_full + 8 * part, j & 1u, abort_flag, p.status);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                if (part == 0) alpha = alpha_row[(j & 1u) * kRows + r];
+                if (part + 1 == kParts) {  // (all of the tile has been multiplied: its probabilities may be overwritten too)
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(o_empty);
+                    if (lane == 0) mbar_arrive(a_empty + 8 * (j & 1u));
                 }
+                const uint64_t alpha2 = pair(alpha, alpha), vi2 = pair(vi, vi);
 #pragma unroll
-                for (uint32_t i = 0; i < 16; i += 2) o[(c0 + i) / 2] = fma2(o[(c0 + i) / 2], alpha2, mul2(pair_bits(y[i], y[i + 1]), vi2));
+                for (uint32_t c0 = 64 * part; c0 < 64 * part + 64; c0 += 16) {
+                    uint32_t y[16];
+                    tmem_ld16_issue(tmem_base + lanes + L::kO + c0, y);
+                    tmem_ld_wait();
+                    if (c0 + 16 == 64 * part + 64) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(o_empty + 8 * part);
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; i += 2) o[(c0 + i) / 2] = fma2(o[(c0 + i) / 2], alpha2, mul2(pair_bits(y[i], y[i + 1]), vi2));
+                }
             }
         }
         ok = ok && mbar_wait(l_full, 0, abort_flag, p.status);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
-            // (the last MMAs and copies are over: K and V are done with)  A row per thread into shared memory, from there as it lies in memory
-            float *rows = reinterpret_cast<float *>(smem) + quarter * 32 * L::kPitch, *mine = rows + lane * L::kPitch;
+            // (the last MMAs and copies are over: K and V are done with)  A row per thread into shared memory
+            float *mine = reinterpret_cast<float *>(smem) + r * L::kPitch;
             const uint64_t lost = pair(kTruncation, kTruncation);
 #pragma unroll
             for (uint32_t i = 0; i < HD; i += 4) {
                 const float2 u = unpair(fma2(o[i / 2], lost, o[i / 2])), w = unpair(fma2(o[i / 2 + 1], lost, o[i / 2 + 1]));
                 *reinterpret_cast<float4 *>(mine + i) = make_float4(u.x, u.y, w.x, w.y);
             }
-            constexpr uint32_t kLanes = HD / 4, kStep = 32 / kLanes;  // lanes per row, rows at a time
-            uint32_t row = row0 + quarter * 32 + lane / kLanes, token = row / p.group, head = row % p.group;
-            const uint32_t d = lane % kLanes * 4;
-            __syncwarp();
-#pragma unroll 8
-            for (uint32_t at = lane / kLanes; at < 32; at += kStep, row += kStep) {
-                const size_t part = ((size_t)token * p.n_heads + kvh * p.group + head) * p.slots + slot;
-                const float4 x = *reinterpret_cast<const float4 *>(rows + at * L::kPitch + d);
-                if (row < n_rows) {
-                    *reinterpret_cast<float4 *>(p.part_o + part * HD + d) = x;
-                    if (d == 0) p.part_ml[part] = make_float2(last_row[quarter * 32 + at] - kProbBits, sum_row[quarter * 32 + at] + sum_row[kRows + quarter * 32 + at]);
-                }
-                for (head += kStep; head >= p.group; head -= p.group) token++;
-            }
         }
     }
 
-    // common exit: nothing of this CTA may still be in flight when its TMEM and shared memory go
+    // nothing of this CTA may still be in flight when its TMEM and shared memory go
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (!*abort_flag && warp < kSumWarp) {
+        // the rows as they lie in memory, sixteen per soft-max warp (which have the registers that the kernel was compiled to)
+        static_assert(kSoftRegs >= kLaunchRegs, "registers");
+        constexpr uint32_t kMine = kRows / kSumWarp;
+        constexpr uint32_t kLanes = HD / 4, kStep = 32 / kLanes;  // lanes per row, rows at a time
+        const float *rows = reinterpret_cast<const float *>(smem);
+        uint32_t at = warp * kMine + lane / kLanes, row = row0 + at, token = row / p.group, head = row - token * p.group;
+        const uint32_t d = lane % kLanes * 4;
+#pragma unroll 8
+        for (uint32_t i = 0; i < kMine / kStep; i++, at += kStep, row += kStep) {
+            if (row < n_rows) {
+                const size_t part = ((size_t)token * p.n_heads + kvh * p.group + head) * p.slots + slot;
+                *reinterpret_cast<float4 *>(p.part_o + part * HD + d) = *reinterpret_cast<const float4 *>(rows + at * L::kPitch + d);
+                if (d == 0) p.part_ml[part] = make_float2(last_row[at] - kProbBits, sum_row[at] + sum_row[kRows + at]);
+            }
+            for (head += kStep; head >= p.group; head -= p.group) token++;
+        }
+    }
+
     if (*abort_flag) {
         // gave up: let MMAs and copies that were already issued drain before the resources are freed
         const long long t0 = clock64();
