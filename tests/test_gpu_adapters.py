@@ -230,7 +230,7 @@ def test_refusals(backend):
 
 def test_a_capture_cannot_grow_the_scratch():
     b = CudaB200Backend(0)
-    c = Call().upload(b)
+    c = Call(batch=70).upload(b)
     b.graph_begin()
     with pytest.raises(YuleGpuError, match="outside the capture"):
         c.run(b)

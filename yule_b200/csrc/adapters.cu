@@ -2,12 +2,21 @@
 //
 // Row i of the batch has adapter a = row_adapter[i] (none if a >= n_adapters: its output is its base), of rank r = min(ranks[a], max_rank):
 //     v_k = Σ_c down[a][k][c] · x[i][c]   (k < r),      out[i][o] = base[i][o] + scales[a] · Σ_k up[a][o][k] · v_k.
-// Two kernels.  The first leaves the sums v of each chunk of columns in the scratch, the second adds the chunks up and multiplies with `up`.  Rows come in tiles; a tile's
-// adapters are its slots: a CTA takes one of them with all the rows of the tile that have it as the columns of the tensor core's second operand, so an
-// adapter is read once per tile whatever the order of the requests, and rows of other adapters are zeros there.  F16 adapters are tf32 numbers as they are: two products
-// per element (of hi and lo of x or v), three for F32 ones.  Sums are added in a fixed order.
+// Rows come in tiles; a tile's adapters are its slots, in the order of their first rows.  A slot's rows are the columns of the tensor core's second operand,
+// so an adapter is read once per tile whatever the order of the requests.  F16 adapters are tf32 numbers as they are: two products per element (with hi and lo of
+// x or v), three for F32 ones.  Sums are added in a fixed order.
+//
+// Decode steps (to 64 rows, tiles of 8): one launch, a cluster of CTAs per slot.  What there is to read is an adapter's 0.1 to 2 MB, so time goes by in latency:
+// a CTA takes a share of the columns for all ranks, writes its sums into every other CTA's shared memory, and has its share of the outputs, whose first rows of `up` and
+// of base it loads before the barrier.
+// Prompts (tiles of 32): two launches, since base and output are most of the traffic and want CTAs of their own; the first as above, the sums joined over a
+// cluster's shared memory into the scratch.
 
 #include <cuda_fp16.h>
+
+#include <utility>
+
+#include <cooperative_groups.h>
 
 #include "internal.h"
 #include "tf32_common.cuh"
@@ -16,58 +25,91 @@ namespace yule {
 
 namespace {
 
-constexpr int kWarps = 4;
+namespace cg = cooperative_groups;
+
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr uint32_t kStepRows = 8, kTileRows = 32, kPassOuts = kWarps * 32;
 
 struct AdapterParams {
     const void *down, *up;
     const uint32_t *ranks, *row_adapter;
     const float *scales, *x, *base;
-    float *out, *sums;  // sums: [row][split][rank_pitch]
-    uint32_t n_adapters, max_rank, n_rows, n_cols, batch, splits, cols_per_split, rank_pitch, slots;
+    float *out, *sums;  // sums (prompts): [row][rank_pitch]
+    uint32_t n_adapters, max_rank, n_rows, n_cols, batch, cols_per_cta, outs_per_cta, rank_pitch;
     size_t x_stride, out_stride;
     bool whole_ranks, whole_outs;  // rows of `up`, and of out and base, are on the boundaries of vectors of four
 };
 
-// The rows of a tile and who is first of its adapter.
-template <int ROWS>
+// A tile's rows by adapter: a lane per row, each warp for itself.
 struct Tile {
-    uint32_t id[ROWS];     // adapter of each row, ~0 for none
-    uint32_t first[ROWS];  // adapters in the order of their first rows
-    uint32_t n;
+    uint32_t id, same, firsts;  // this row's adapter (~0: none), the rows that share it, the first row of each adapter
 };
-template <int ROWS>
-__device__ __forceinline__ void read_tile(const AdapterParams &p, uint32_t row0, Tile<ROWS> &tile) {
-    static_assert(ROWS <= 32, "a lane per row");
-    if (threadIdx.x < 32) {
-        const uint32_t lane = threadIdx.x, row = row0 + lane;
-        uint32_t id = lane < ROWS && row < p.batch ? __ldg(p.row_adapter + row) : ~0u;
-        if (id >= p.n_adapters) id = ~0u;
-        const uint32_t same = __match_any_sync(0xffffffffu, id), firsts = __ballot_sync(0xffffffffu, id != ~0u && (uint32_t)__ffs(same) == lane + 1);
-        if (lane < ROWS) tile.id[lane] = id;
-        if (firsts >> lane & 1u) tile.first[__popc(firsts & ((1u << lane) - 1))] = id;
-        if (lane == 0) tile.n = __popc(firsts);
+template <uint32_t ROWS>
+__device__ __forceinline__ Tile read_tile(const AdapterParams &p, uint32_t row0) {
+    const uint32_t lane = threadIdx.x & 31, row = row0 + lane;
+    Tile t;
+    t.id = lane < ROWS && row < p.batch ? __ldg(p.row_adapter + row) : ~0u;
+    if (t.id >= p.n_adapters) t.id = ~0u;
+    t.same = __match_any_sync(0xffffffffu, t.id);
+    t.firsts = __ballot_sync(0xffffffffu, t.id != ~0u && (uint32_t)__ffs(t.same) == lane + 1);
+    return t;
+}
+// Adapter and rows of a slot, the rows in `list`, one of the warp's own.
+struct Slot {
+    uint32_t adapter, n;
+};
+__device__ __forceinline__ Slot read_slot(const Tile &t, uint32_t slot, uint8_t *list) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t f = t.firsts;
+    for (uint32_t i = 0; i < slot; i++) f &= f - 1;
+    const int first = __ffs(f) - 1;
+    const uint32_t mask = __shfl_sync(0xffffffffu, t.same, first);
+    __syncwarp();
+    if (mask >> lane & 1u) list[__popc(mask & ((1u << lane) - 1))] = (uint8_t)lane;
+    __syncwarp();
+    return {__shfl_sync(0xffffffffu, t.id, first), (uint32_t)__popc(mask)};
+}
+// Rows without an adapter: their base, outputs [o0, o1).
+template <uint32_t ROWS>
+__device__ __forceinline__ void copy_base(const AdapterParams &p, const Tile &t, uint32_t row0, uint32_t o0, uint32_t o1) {
+    if (p.base == p.out) return;
+    for (uint32_t none = __ballot_sync(0xffffffffu, t.id == ~0u && (threadIdx.x & 31) < ROWS && row0 + (threadIdx.x & 31) < p.batch); none; none &= none - 1) {
+        const size_t at = (size_t)(row0 + __ffs(none) - 1) * p.out_stride;
+        if (p.whole_outs)
+            for (uint32_t o = o0 + 4 * threadIdx.x; o < o1; o += 4 * kThreads) *reinterpret_cast<float4 *>(p.out + at + o) = *reinterpret_cast<const float4 *>(p.base + at + o);
+        else
+            for (uint32_t o = o0 + threadIdx.x; o < o1; o += kThreads) p.out[at + o] = p.base[at + o];
     }
-    __syncthreads();
 }
 
-// Four elements of an adapter's row from `at` on, of which `n` are there, as fp32.
+// Four elements of an adapter's row from `at` on, of which `n` are there, as they lie and as fp32.
 template <typename T>
-__device__ __forceinline__ float4 four(const T *at, int n, bool whole);
+struct Four;
 template <>
-__device__ __forceinline__ float4 four<float>(const float *at, int n, bool whole) {
-    if (whole && n >= 4) return __ldg(reinterpret_cast<const float4 *>(at));
-    return make_float4(n > 0 ? __ldg(at) : 0.f, n > 1 ? __ldg(at + 1) : 0.f, n > 2 ? __ldg(at + 2) : 0.f, n > 3 ? __ldg(at + 3) : 0.f);
-}
+struct Four<float> {
+    float4 v;
+    __device__ __forceinline__ void load(const float *at, int n, bool whole) {
+        if (whole && n >= 4) v = __ldg(reinterpret_cast<const float4 *>(at));
+        else v = make_float4(n > 0 ? __ldg(at) : 0.f, n > 1 ? __ldg(at + 1) : 0.f, n > 2 ? __ldg(at + 2) : 0.f, n > 3 ? __ldg(at + 3) : 0.f);
+    }
+    __device__ __forceinline__ float4 get() const { return v; }
+};
 template <>
-__device__ __forceinline__ float4 four<__half>(const __half *at, int n, bool whole) {
-    if (whole && n >= 4) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(at));
+struct Four<__half> {
+    uint2 v;
+    __device__ __forceinline__ void load(const __half *at, int n, bool whole) {
+        if (whole && n >= 4) v = __ldg(reinterpret_cast<const uint2 *>(at));
+        else {
+            const unsigned short *bits = reinterpret_cast<const unsigned short *>(at);
+            auto one = [&](int i) -> uint32_t { return n > i ? __ldg(bits + i) : 0u; };
+            v = make_uint2(one(0) | one(1) << 16, one(2) | one(3) << 16);
+        }
+    }
+    __device__ __forceinline__ float4 get() const {
         const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
         return make_float4(a.x, a.y, b.x, b.y);
     }
-    auto one = [&](int i) { return n > i ? __half2float(__ldg(at + i)) : 0.f; };
-    return make_float4(one(0), one(1), one(2), one(3));
-}
+};
 
 // d += a · b over two steps of eight: this lane's four elements of the operands' rows g (a) and g + 8 (b), and of the second operand's column g.
 template <bool EXACT>  // a and b are tf32 numbers
@@ -90,210 +132,418 @@ __device__ __forceinline__ void split4(const float4 &v, uint4 &hi, uint4 &lo) {
     split_tf32(v.x, hi.x, lo.x), split_tf32(v.y, hi.y, lo.y), split_tf32(v.z, hi.z, lo.z), split_tf32(v.w, hi.w, lo.w);
 }
 
-// v of a tile's rows over a chunk of columns: 16·RANKS rows of `down` at a time, rows of x in eights as columns.  A warp takes 64 columns in turn with the others.
-template <typename T, int ROWS, int RANKS>
-__global__ void __launch_bounds__(kWarps * 32) adapter_down_kernel(const __grid_constant__ AdapterParams p) {
-    __shared__ Tile<ROWS * 8> tile;
-    __shared__ float meet[kWarps][ROWS * 8][RANKS * 16 + 1];
+__device__ __forceinline__ void store4(const AdapterParams &p, size_t at, uint32_t o, const float4 &b, const float (&d)[4], float scale) {
+    const float4 v = make_float4(fmaf(scale, d[0], b.x), fmaf(scale, d[1], b.y), fmaf(scale, d[2], b.z), fmaf(scale, d[3], b.w));
+    float *to = p.out + at + o;
+    if (p.whole_outs) {
+        if (o < p.n_rows) *reinterpret_cast<float4 *>(to) = v;
+    } else {
+        if (o < p.n_rows) to[0] = v.x;
+        if (o + 1 < p.n_rows) to[1] = v.y;
+        if (o + 2 < p.n_rows) to[2] = v.z;
+        if (o + 3 < p.n_rows) to[3] = v.w;
+    }
+}
+__device__ __forceinline__ float4 load4(const AdapterParams &p, size_t at, uint32_t o, bool there) {  // (not by the read-only path: it can be the output)
+    const float *from = p.base + at + o;
+    if (p.whole_outs) return there && o < p.n_rows ? *reinterpret_cast<const float4 *>(from) : make_float4(0.f, 0.f, 0.f, 0.f);
+    return make_float4(there && o < p.n_rows ? from[0] : 0.f, there && o + 1 < p.n_rows ? from[1] : 0.f, there && o + 2 < p.n_rows ? from[2] : 0.f, there && o + 3 < p.n_rows ? from[3] : 0.f);
+}
+// Rows o .. o + 3 of `up`, this lane's elements of step j: what the lane has of the first operand, in an order that gives it four consecutive outputs.
+template <typename T>
+__device__ __forceinline__ void load_up(const AdapterParams &p, const T *up, uint32_t o, uint32_t j, uint32_t rank, Four<T> (&u)[4]) {
+    const uint32_t k = 16 * j + 4 * (threadIdx.x & 3);
+#pragma unroll
+    for (int i = 0; i < 4; i++) u[i].load(up + (size_t)(o + i) * p.max_rank + k, o + i < p.n_rows ? (int)rank - (int)k : 0, p.whole_ranks);
+}
+// The terms of v lie in rows of so many words: eight lanes of a 16-byte load are in different banks.
+__host__ __device__ __forceinline__ uint32_t v_pitch(uint32_t max_rank) { return (max_rank + 31) / 32 * 32 + 16; }
+
+// A decode step's slot: grid x = the cluster, y = slots, z = tiles.
+template <typename T, int RANKS>
+__global__ void __launch_bounds__(kThreads, 2) adapter_step_kernel(const __grid_constant__ AdapterParams p) {
+    extern __shared__ __align__(16) float got[];  // sums of v: [CTA][row][rank_pitch], then v's terms: hi, lo: [row][pitch]
+    __shared__ float meet[kWarps][kStepRows][RANKS * 16 + 1];
+    __shared__ uint8_t lists[kWarps][32];
+    cg::cluster_group cluster = cg::this_cluster();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t row0 = blockIdx.x * ROWS * 8, split = blockIdx.z;
+    const uint32_t ctas = gridDim.x, cta = blockIdx.x, row0 = blockIdx.z * kStepRows, slot_at = blockIdx.y;
+    const uint32_t out0 = cta * p.outs_per_cta, out1 = min(out0 + p.outs_per_cta, p.n_rows);
+    auto started = cluster.barrier_arrive();  // (waited for before anything is written to another CTA)
     yule_pdl_launch_dependents();
     yule_pdl_wait();
-    read_tile(p, row0, tile);
-    const uint32_t col0 = split * p.cols_per_split, col1 = min(col0 + p.cols_per_split, p.n_cols);
-    for (uint32_t slot = blockIdx.y; slot < tile.n; slot += p.slots) {
-        const uint32_t a = tile.first[slot], rank = min(__ldg(p.ranks + a), p.max_rank);
-        const T *down = static_cast<const T *>(p.down) + (size_t)a * p.max_rank * p.n_cols;
-        bool mine[ROWS];
+    const uint32_t near_rank = lane < p.n_adapters ? __ldg(p.ranks + lane) : 0u;  // (beside the rows' adapters, not behind them)
+    const Tile tile = read_tile<kStepRows>(p, row0);
+    if (slot_at == 0) copy_base<kStepRows>(p, tile, row0, out0, out1);
+    if (slot_at >= __popc(tile.firsts)) {  // (the same for all the cluster)
+        cluster.barrier_wait(std::move(started));
+        return;
+    }
+    const uint8_t *rows = lists[warp];
+    const Slot slot = read_slot(tile, slot_at, lists[warp]);
+    const uint32_t near = __shfl_sync(0xffffffffu, near_rank, slot.adapter & 31), rank = min(slot.adapter < 32 ? near : __ldg(p.ranks + slot.adapter), p.max_rank);
+    const float scale = __ldg(p.scales + slot.adapter);
+    const T *down = static_cast<const T *>(p.down) + (size_t)slot.adapter * p.max_rank * p.n_cols, *up = static_cast<const T *>(p.up) + (size_t)slot.adapter * p.n_rows * p.max_rank;
+    const uint32_t share = p.cols_per_cta / kWarps, col0 = (cta * kWarps + warp) * share, col1 = min(col0 + share, p.n_cols);
+    const float *x = p.x + (size_t)(row0 + rows[g < slot.n ? g : 0]) * p.x_stride;
+    bool first = true;
+    for (uint32_t k0 = 0; k0 < rank; k0 += RANKS * 16) {
+        constexpr int kSteps = RANKS == 4 && sizeof(T) == 4 ? 2 : 4;  // steps whose loads are under way together
+        float sum[RANKS][4] = {};
+        for (uint32_t base = col0; base < col1; base += 16 * kSteps) {
+            float4 xv[kSteps];
+            Four<T> w[kSteps][RANKS][2];
 #pragma unroll
-        for (int n = 0; n < ROWS; n++) mine[n] = tile.id[8 * n + g] == a;
-        for (uint32_t k0 = 0; k0 < rank; k0 += RANKS * 16) {
-            float sum[RANKS][ROWS][4];
+            for (int j = 0; j < kSteps; j++) {
+                const uint32_t c = base + 16 * j + 4 * t;
+                const bool in = c < col1;
+                xv[j] = in && g < slot.n ? __ldg(reinterpret_cast<const float4 *>(x + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int r = 0; r < RANKS; r++)
-#pragma unroll
-                for (int n = 0; n < ROWS; n++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) sum[r][n][e] = 0.f;
-            for (uint32_t base = col0 + warp * 64; base < col1; base += kWarps * 64) {
-                // (the tensor core truncates what it adds to: sums of 64 columns, added up in fp32)
-                float d[RANKS][ROWS][4];
-#pragma unroll
-                for (int r = 0; r < RANKS; r++)
-#pragma unroll
-                    for (int n = 0; n < ROWS; n++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) d[r][n][e] = 0.f;
-#pragma unroll
-                for (uint32_t j = 0; j < 4; j++) {
-                    const uint32_t c = base + 16 * j + 4 * t;
-                    const bool in = c < col1;
-                    uint4 hi[ROWS], lo[ROWS];
-#pragma unroll
-                    for (int n = 0; n < ROWS; n++)
-                        split4(in && mine[n] ? __ldg(reinterpret_cast<const float4 *>(p.x + (size_t)(row0 + 8 * n + g) * p.x_stride + c)) : make_float4(0.f, 0.f, 0.f, 0.f), hi[n], lo[n]);
-#pragma unroll
-                    for (int r = 0; r < RANKS; r++) {
-                        const uint32_t k = k0 + 16 * r + g;
-                        const float4 u = four(down + (size_t)k * p.n_cols + c, in && k < rank ? 4 : 0, true), v = four(down + (size_t)(k + 8) * p.n_cols + c, in && k + 8 < rank ? 4 : 0, true);
-#pragma unroll
-                        for (int n = 0; n < ROWS; n++) multiply<sizeof(T) == 2>(d[r][n], u, v, hi[n], lo[n]);
-                    }
+                for (int r = 0; r < RANKS; r++) {
+                    const uint32_t k = k0 + 16 * r + g;
+                    w[j][r][0].load(down + (size_t)k * p.n_cols + c, in && k < rank ? 4 : 0, true);
+                    w[j][r][1].load(down + (size_t)(k + 8) * p.n_cols + c, in && k + 8 < rank ? 4 : 0, true);
                 }
-#pragma unroll
-                for (int r = 0; r < RANKS; r++)
-#pragma unroll
-                    for (int n = 0; n < ROWS; n++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) sum[r][n][e] += d[r][n][e];
             }
-            __syncthreads();
+            // (the tensor core truncates what it adds to: sums of 32 or 64 columns, added up in fp32)
+            float d[RANKS][4] = {};
+#pragma unroll
+            for (int j = 0; j < kSteps; j++) {
+                uint4 hi, lo;
+                split4(xv[j], hi, lo);
+#pragma unroll
+                for (int r = 0; r < RANKS; r++) multiply<sizeof(T) == 2>(d[r], w[j][r][0].get(), w[j][r][1].get(), hi, lo);
+            }
 #pragma unroll
             for (int r = 0; r < RANKS; r++)
 #pragma unroll
-                for (int n = 0; n < ROWS; n++)
+                for (int e = 0; e < 4; e++) sum[r][e] += d[r][e];
+        }
+        if (k0) __syncthreads();
 #pragma unroll
-                    for (int e = 0; e < 4; e++) meet[warp][8 * n + 2 * t + (e & 1)][16 * r + g + 8 * (e >> 1)] = sum[r][n][e];
-            __syncthreads();
-            for (uint32_t i = threadIdx.x; i < ROWS * 8 * RANKS * 16; i += kWarps * 32) {
-                const uint32_t row = i / (RANKS * 16), k = i % (RANKS * 16);
-                if (tile.id[row] != a || k0 + k >= rank) continue;
-                float v = 0.f;
+        for (int r = 0; r < RANKS; r++)
 #pragma unroll
-                for (int w = 0; w < kWarps; w++) v += meet[w][row][k];
-                p.sums[((size_t)(row0 + row) * p.splits + split) * p.rank_pitch + k0 + k] = v;
-            }
+            for (int e = 0; e < 4; e++) meet[warp][2 * t + (e & 1)][16 * r + g + 8 * (e >> 1)] = sum[r][e];
+        __syncthreads();
+        if (first) cluster.barrier_wait(std::move(started));
+        first = false;
+        for (uint32_t i = threadIdx.x; i < slot.n * RANKS * 16 * 4; i += kThreads) {  // four threads per sum, each for a fourth of the CTAs
+            const uint32_t row = i / (RANKS * 64), k = i / 4 % (RANKS * 16);
+            if (k0 + k >= rank) continue;
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) v += meet[w][row][k];
+            for (uint32_t c = i & 3u; c < ctas; c += 4) cluster.map_shared_rank(got, c)[(cta * kStepRows + row) * p.rank_pitch + k0 + k] = v;
+        }
+    }
+    if (first) cluster.barrier_wait(std::move(started));
+    auto summed = cluster.barrier_arrive();
+    const uint32_t steps = (rank + 15) / 16;
+    uint32_t o = out0 + warp * 32 + 4 * g;
+    const bool mine[2] = {2 * t < slot.n, 2 * t + 1 < slot.n};
+    size_t at[2];
+    float4 b[2];
+    Four<T> u[4];
+    const uint32_t end = out0 + p.outs_per_cta;
+#pragma unroll
+    for (int c = 0; c < 2; c++) at[c] = (size_t)(row0 + rows[mine[c] ? 2 * t + c : 0]) * p.out_stride, b[c] = load4(p, at[c], o, mine[c] && o < end);
+    load_up(p, up, o, 0, o < end ? rank : 0, u);
+    cluster.barrier_wait(std::move(summed));
+    const uint32_t pitch = v_pitch(p.max_rank);
+    uint32_t *v_hi = reinterpret_cast<uint32_t *>(got + ctas * kStepRows * p.rank_pitch), *v_lo = v_hi + kStepRows * pitch;
+    for (uint32_t i = threadIdx.x; i < slot.n * steps * 16; i += kThreads) {
+        const uint32_t r = i / (steps * 16), k = i % (steps * 16);
+        float v = 0.f;
+        if (k < rank)
+            for (uint32_t c = 0; c < ctas; c++) v += got[(c * kStepRows + r) * p.rank_pitch + k];
+        split_tf32(v, v_hi[r * pitch + k], v_lo[r * pitch + k]);
+    }
+    __syncthreads();
+    for (; o < end; o += kPassOuts) {
+        const uint32_t next = o + kPassOuts;
+        float4 bn[2];
+#pragma unroll
+        for (int c = 0; c < 2; c++) bn[c] = load4(p, at[c], next, mine[c] && next < end);
+        float d[2][4] = {};
+        for (uint32_t j = 0; j < steps; j++) {
+            Four<T> un[4];
+            const bool last = j + 1 == steps;
+            load_up(p, up, last ? next : o, last ? 0 : j + 1, last && next >= end ? 0 : rank, un);
+            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+            if (g < slot.n) hi = *reinterpret_cast<const uint4 *>(v_hi + g * pitch + 16 * j + 4 * t), lo = *reinterpret_cast<const uint4 *>(v_lo + g * pitch + 16 * j + 4 * t);
+            multiply<sizeof(T) == 2>(d[0], u[0].get(), u[1].get(), hi, lo);
+            multiply<sizeof(T) == 2>(d[1], u[2].get(), u[3].get(), hi, lo);
+#pragma unroll
+            for (int i = 0; i < 4; i++) u[i] = un[i];
+        }
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const float four_of[4] = {d[0][c], d[0][2 + c], d[1][c], d[1][2 + c]};
+            if (mine[c]) store4(p, at[c], o, b[c], four_of, scale);
+            b[c] = bn[c];
         }
     }
 }
 
-// out of a tile's rows for 32 outputs a warp: rows of `up` as rows of the first operand, in an order that gives a lane four consecutive outputs.
-template <typename T, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32) adapter_up_kernel(const __grid_constant__ AdapterParams p) {
-    extern __shared__ __align__(16) uint32_t v_terms[];  // hi, then lo: [row][pitch]
-    __shared__ Tile<ROWS * 8> tile;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t row0 = blockIdx.x * ROWS * 8, pitch = (p.max_rank + 31) / 32 * 32 + 16, o = (blockIdx.z * kWarps + warp) * 32 + 4 * g;
-    uint32_t *v_hi = v_terms, *v_lo = v_terms + ROWS * 8 * pitch;
+// ── prompts ─────────────────────────────────────────────────────────────────────────────────────
+// cp.async of W bytes, zeros where there is nothing.
+template <int W>
+__device__ __forceinline__ void copy_async(uint32_t to, const void *from, bool there) {
+    const int bytes = there ? W : 0;
+    if (W == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+
+template <typename T>
+struct DownLayout {
+    static constexpr uint32_t kCols = 64, kRanks = 64, kStages = 3;
+    static constexpr uint32_t kXPitch = (kCols + 16) * 4, kDPitch = (kCols + 16) * sizeof(T);  // bytes: 16- or 8-byte loads of eight rows in different banks
+    static constexpr uint32_t kX = kTileRows * kXPitch, kStage = kX + kRanks * kDPitch;
+    static constexpr uint32_t kMeet = 4 * kTileRows * (kRanks + 1) * 4, kSum = kTileRows * kRanks * 4;
+    static constexpr uint32_t kRing = kStages * kStage, kBytes = (kRing > kMeet ? kRing : kMeet) + kSum;
+};
+
+// v of a tile's slots, 64 ranks at a time: grid x = tiles × the cluster (a share of the columns per CTA), y = slots.  A warp has 32 ranks and 16 of each 64 columns.
+template <typename T, int W>
+__global__ void __launch_bounds__(kThreads, 2) adapter_down_kernel(const __grid_constant__ AdapterParams p) {
+    using L = DownLayout<T>;
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ uint8_t lists[kWarps][32];
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, part = warp & 3, half = warp >> 2;
+    const uint32_t ctas = cluster.num_blocks(), cta = cluster.block_rank(), row0 = blockIdx.x / ctas * kTileRows;
+    float *meet = reinterpret_cast<float *>(ring), *mine = reinterpret_cast<float *>(ring + L::kBytes - L::kSum);
     yule_pdl_launch_dependents();
     yule_pdl_wait();
-    read_tile(p, row0, tile);
-    auto store = [&](uint32_t row, const float (&d)[4], float scale) {
-        const float *from = p.base + (size_t)row * p.out_stride + o;
-        float *to = p.out + (size_t)row * p.out_stride + o;
-        if (p.whole_outs) {
-            if (o >= p.n_rows) return;
-            const float4 b = *reinterpret_cast<const float4 *>(from);
-            *reinterpret_cast<float4 *>(to) = make_float4(fmaf(scale, d[0], b.x), fmaf(scale, d[1], b.y), fmaf(scale, d[2], b.z), fmaf(scale, d[3], b.w));
-        } else {
+    const Tile tile = read_tile<kTileRows>(p, row0);
+    const uint32_t n_slots = __popc(tile.firsts), col0 = cta * p.cols_per_cta, col1 = min(col0 + p.cols_per_cta, p.n_cols), to = (uint32_t)__cvta_generic_to_shared(ring);
+    const uint32_t n_stages = col0 < col1 ? (col1 - col0 + L::kCols - 1) / L::kCols : 0;
+    const uint8_t *rows = lists[warp];
+    for (uint32_t s = blockIdx.y; s < n_slots; s += gridDim.y) {
+        const Slot slot = read_slot(tile, s, lists[warp]);
+        const uint32_t rank = min(__ldg(p.ranks + slot.adapter), p.max_rank);
+        const T *down = static_cast<const T *>(p.down) + (size_t)slot.adapter * p.max_rank * p.n_cols;
+        const float *from[2];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (o + i < p.n_rows) to[i] = fmaf(scale, d[i], from[i]);
+        for (int i = 0; i < 2; i++) {
+            const uint32_t r = threadIdx.x / 16 + 16 * i;
+            from[i] = p.x + (size_t)(row0 + rows[r < slot.n ? r : 0]) * p.x_stride;
         }
-    };
-    // rows without an adapter: their base
-    if (blockIdx.y == 0 && p.base != p.out)
+        for (uint32_t k0 = 0; k0 < rank; k0 += L::kRanks) {
+            auto load = [&](uint32_t i) {
+                if (i < n_stages) {
+                    const uint32_t stage = to + i % L::kStages * L::kStage, c0 = col0 + i * L::kCols;
 #pragma unroll
-        for (int n = 0; n < ROWS; n++)
+                    for (int n = 0; n < 2; n++) {
+                        const uint32_t r = threadIdx.x / 16 + 16 * n, c = threadIdx.x % 16 * 4;
+                        const bool there = r < slot.n && c0 + c < col1;
+                        copy_async<16>(stage + r * L::kXPitch + c * 4, there ? from[n] + c0 + c : p.x, there);
+                    }
+                    constexpr uint32_t per_row = L::kCols * sizeof(T) / W;
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const uint32_t r = 8 * n + 2 * t + c;
-                const float none[4] = {0.f, 0.f, 0.f, 0.f};
-                if (tile.id[r] == ~0u && row0 + r < p.batch) store(row0 + r, none, 0.f);
+                    for (uint32_t n = 0; n < L::kRanks * per_row / kThreads; n++) {
+                        const uint32_t at = threadIdx.x + n * kThreads, k = at / per_row, c = at % per_row * (W / sizeof(T));
+                        const bool there = k0 + k < rank && c0 + c < col1;
+                        copy_async<W>(stage + L::kX + k * L::kDPitch + c * sizeof(T), there ? down + (size_t)(k0 + k) * p.n_cols + c0 + c : down, there);
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            float sum[2][4][4] = {}, d[2][4][4] = {};
+            const bool used = k0 + 32 * half < rank;
+#pragma unroll
+            for (uint32_t i = 0; i + 1 < L::kStages; i++) load(i);
+            for (uint32_t i = 0; i < n_stages; i++) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
+                __syncthreads();  // (the stage is there, and the one before has been read by all)
+                load(i + L::kStages - 1);
+                const uint8_t *stage = ring + i % L::kStages * L::kStage;
+                if (used) {
+                    Four<T> w[2][2];
+#pragma unroll
+                    for (int r = 0; r < 2; r++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+                            w[r][h].v = *reinterpret_cast<const decltype(w[r][h].v) *>(stage + L::kX + (32 * half + 16 * r + 8 * h + g) * L::kDPitch + (16 * part + 4 * t) * sizeof(T));
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        if (8 * n >= slot.n) break;
+                        uint4 hi, lo;
+                        split4(*reinterpret_cast<const float4 *>(stage + (8 * n + g) * L::kXPitch + (16 * part + 4 * t) * 4), hi, lo);
+#pragma unroll
+                        for (int r = 0; r < 2; r++) multiply<sizeof(T) == 2>(d[r][n], w[r][0].get(), w[r][1].get(), hi, lo);
+                    }
+                    if ((i & 3) == 3 || i + 1 == n_stages) {  // (the tensor core truncates what it adds to: sums of 64 columns, added up in fp32)
+#pragma unroll
+                        for (int r = 0; r < 2; r++)
+#pragma unroll
+                            for (int n = 0; n < 4; n++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) sum[r][n][e] += d[r][n][e], d[r][n][e] = 0.f;
+                    }
+                }
             }
-    for (uint32_t slot = blockIdx.y; slot < tile.n; slot += p.slots) {
-        const uint32_t a = tile.first[slot], rank = min(__ldg(p.ranks + a), p.max_rank), steps = (rank + 15) / 16;
-        const float scale = __ldg(p.scales + a);
-        const T *up = static_cast<const T *>(p.up) + (size_t)a * p.n_rows * p.max_rank;
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) meet[(part * kTileRows + 8 * n + 2 * t + (e & 1)) * (L::kRanks + 1) + 32 * half + 16 * r + g + 8 * (e >> 1)] = sum[r][n][e];
+            __syncthreads();
+            const uint32_t n_ranks = min(rank - k0, L::kRanks);
+            for (uint32_t i = threadIdx.x; i < slot.n * L::kRanks; i += kThreads) {
+                const uint32_t r = i / L::kRanks, k = i % L::kRanks;
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; w++) v += meet[(w * kTileRows + r) * (L::kRanks + 1) + k];
+                mine[i] = v;
+            }
+            cluster.sync();
+            for (uint32_t i = cta * kThreads + threadIdx.x; i < slot.n * L::kRanks; i += ctas * kThreads) {
+                const uint32_t r = i / L::kRanks, k = i % L::kRanks;
+                if (k >= n_ranks) continue;
+                float v = 0.f;
+                for (uint32_t c = 0; c < ctas; c++) v += cluster.map_shared_rank(mine, c)[i];
+                p.sums[(size_t)(row0 + rows[r]) * p.rank_pitch + k0 + k] = v;
+            }
+            cluster.sync();  // (the other CTAs have read this one's sums)
+        }
+    }
+}
+
+// out of a tile's slots, a share of the outputs per CTA: grid x = tiles, y = slots, z = shares.  32 outputs a warp and pass, base loaded before the products.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) adapter_up_kernel(const __grid_constant__ AdapterParams p) {
+    extern __shared__ __align__(16) uint32_t v_hi[];  // hi, then lo: [row][pitch]
+    __shared__ uint8_t lists[kWarps][32];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t row0 = blockIdx.x * kTileRows, out0 = blockIdx.z * p.outs_per_cta, end = min(out0 + p.outs_per_cta, p.n_rows), pitch = v_pitch(p.max_rank);
+    uint32_t *v_lo = v_hi + kTileRows * pitch;
+    yule_pdl_launch_dependents();
+    yule_pdl_wait();
+    const Tile tile = read_tile<kTileRows>(p, row0);
+    if (blockIdx.y == 0) copy_base<kTileRows>(p, tile, row0, out0, end);
+    const uint32_t n_slots = __popc(tile.firsts);
+    const uint8_t *rows = lists[warp];
+    for (uint32_t s = blockIdx.y; s < n_slots; s += gridDim.y) {
+        const Slot slot = read_slot(tile, s, lists[warp]);
+        const uint32_t rank = min(__ldg(p.ranks + slot.adapter), p.max_rank), steps = (rank + 15) / 16;
+        const float scale = __ldg(p.scales + slot.adapter);
+        const T *up = static_cast<const T *>(p.up) + (size_t)slot.adapter * p.n_rows * p.max_rank;
         __syncthreads();  // (the slot before has read its sums)
-        for (uint32_t i = threadIdx.x; i < ROWS * 8 * steps * 16; i += kWarps * 32) {
+        for (uint32_t i = threadIdx.x; i < kTileRows * steps * 16; i += kThreads) {
             const uint32_t r = i / (steps * 16), k = i % (steps * 16);
-            float v = 0.f;
-            if (tile.id[r] == a && k < rank)
-                for (uint32_t s = 0; s < p.splits; s++) v += __ldcg(p.sums + ((size_t)(row0 + r) * p.splits + s) * p.rank_pitch + k);
+            const float v = r < slot.n && k < rank ? __ldcg(p.sums + (size_t)(row0 + rows[r]) * p.rank_pitch + k) : 0.f;
             split_tf32(v, v_hi[r * pitch + k], v_lo[r * pitch + k]);
         }
         __syncthreads();
-        float d[2][ROWS][4];
+        for (uint32_t o = out0 + warp * 32 + 4 * g; o - 4 * g < end; o += kPassOuts) {
+            float4 b[4][2];
 #pragma unroll
-        for (int c = 0; c < 2; c++)
+            for (int n = 0; n < 4; n++)
 #pragma unroll
-            for (int n = 0; n < ROWS; n++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) d[c][n][e] = 0.f;
+                for (int c = 0; c < 2; c++) {
+                    const uint32_t r = 8 * n + 2 * t + c;
+                    b[n][c] = load4(p, (size_t)(row0 + rows[r < slot.n ? r : 0]) * p.out_stride, o, r < slot.n);
+                }
+            float d[2][4][4] = {};
 #pragma unroll 2
-        for (uint32_t j = 0; j < steps; j++) {
-            const uint32_t k = 16 * j + 4 * t;
-            const int there = (int)rank - (int)k;
-            float4 u[4];
+            for (uint32_t j = 0; j < steps; j++) {
+                Four<T> u[4];
+                load_up(p, up, o, j, rank, u);
 #pragma unroll
-            for (int i = 0; i < 4; i++) u[i] = four(up + (size_t)(o + i) * p.max_rank + k, o + i < p.n_rows ? there : 0, p.whole_ranks);
-#pragma unroll
-            for (int n = 0; n < ROWS; n++) {
-                const uint4 hi = *reinterpret_cast<const uint4 *>(v_hi + (8 * n + g) * pitch + k), lo = *reinterpret_cast<const uint4 *>(v_lo + (8 * n + g) * pitch + k);
-                multiply<sizeof(T) == 2>(d[0][n], u[0], u[1], hi, lo);
-                multiply<sizeof(T) == 2>(d[1][n], u[2], u[3], hi, lo);
+                for (int n = 0; n < 4; n++) {
+                    if (8 * n >= slot.n) break;
+                    const uint4 hi = *reinterpret_cast<const uint4 *>(v_hi + (8 * n + g) * pitch + 16 * j + 4 * t), lo = *reinterpret_cast<const uint4 *>(v_lo + (8 * n + g) * pitch + 16 * j + 4 * t);
+                    multiply<sizeof(T) == 2>(d[0][n], u[0].get(), u[1].get(), hi, lo);
+                    multiply<sizeof(T) == 2>(d[1][n], u[2].get(), u[3].get(), hi, lo);
+                }
             }
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const uint32_t r = 8 * n + 2 * t + c;
+                    const float four_of[4] = {d[0][n][c], d[0][n][2 + c], d[1][n][c], d[1][n][2 + c]};
+                    if (r < slot.n) store4(p, (size_t)(row0 + rows[r]) * p.out_stride, o, b[n][c], four_of, scale);
+                }
         }
-#pragma unroll
-        for (int n = 0; n < ROWS; n++)
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const uint32_t r = 8 * n + 2 * t + c;
-                const float four_of[4] = {d[0][n][c], d[0][n][2 + c], d[1][n][c], d[1][n][2 + c]};
-                if (tile.id[r] == a) store(row0 + r, four_of, scale);
-            }
     }
 }
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+uint32_t rank_pitch(const AdapterBatch &a) { return (a.max_rank + 3) / 4 * 4; }
+bool is_step(const AdapterBatch &a) { return a.batch <= 64; }
 
-// Tiles of 32 rows for prompts, of 8 with a slot per row for decode steps.
-uint32_t tile_rows(const AdapterBatch &a) { return a.batch > 64 ? 32 : 8; }
-uint32_t splits_of(const AdapterBatch &a, int sm_count) {
-    const uint32_t slots = tile_rows(a) == 8 ? a.batch : ceil_div(a.batch, 32);
-    const uint32_t want = ceil_div(3 * (uint64_t)sm_count, slots), most = ceil_div(a.n_cols, kWarps * 64);
-    return want < most ? want : most;
+cudaError_t launch_cluster(void (*kern)(AdapterParams), dim3 grid, uint32_t ctas, size_t smem, bool pdl, cudaStream_t s, const AdapterParams &p) {
+    cudaError_t e;
+    if (ctas > 8 && (e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+    if (smem > 24 * 1024 && (e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid, cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 2 : 1;
+    return launch_config(cfg, kern, p);
 }
 
 template <typename T>
-cudaError_t launch_typed(const AdapterBatch &a, AdapterParams p, cudaStream_t s, uint64_t *launches) {
-    const uint32_t rows = tile_rows(a), tiles = ceil_div(a.batch, rows);
-    const dim3 block(kWarps * 32), down(tiles, p.slots, p.splits), up(tiles, p.slots, ceil_div(a.n_rows, kWarps * 32));
-    if (up.z > 65535) return cudaErrorInvalidValue;
-    cudaError_t e;
-    if (rows == 8)
-        e = a.max_rank <= 16 ? launch_kernel(adapter_down_kernel<T, 1, 1>, down, block, 0, s, a.pdl, p) : launch_kernel(adapter_down_kernel<T, 1, 4>, down, block, 0, s, a.pdl, p);
-    else
-        e = a.max_rank <= 16 ? launch_kernel(adapter_down_kernel<T, 4, 1>, down, block, 0, s, a.pdl, p) : launch_kernel(adapter_down_kernel<T, 4, 4>, down, block, 0, s, a.pdl, p);
+cudaError_t launch_step(const AdapterBatch &a, AdapterParams p, cudaStream_t s, uint64_t *launches) {
+    const uint32_t tiles = ceil_div(a.batch, kStepRows), slots = a.batch < kStepRows ? a.batch : kStepRows;
+    const uint32_t ctas = tiles * slots <= 16 ? 16 : 8;
+    p.cols_per_cta = ceil_div(a.n_cols, ctas * kWarps * 16) * kWarps * 16;
+    p.outs_per_cta = ceil_div(a.n_rows, ctas * 32) * 32;
+    const size_t smem = (size_t)kStepRows * (ctas * p.rank_pitch + 2 * v_pitch(a.max_rank)) * sizeof(float);
+    auto kern = a.max_rank <= 16 ? adapter_step_kernel<T, 1> : adapter_step_kernel<T, 4>;
+    const cudaError_t e = launch_cluster(kern, dim3(ctas, slots, tiles), ctas, smem, a.pdl, s, p);
+    if (e == cudaSuccess) ++*launches;
+    return e;
+}
+
+template <typename T>
+cudaError_t launch_prompts(const AdapterBatch &a, AdapterParams p, cudaStream_t s, uint64_t *launches) {
+    using L = DownLayout<T>;
+    const uint32_t tiles = ceil_div(a.batch, kTileRows), slots = a.n_adapters < 4 ? a.n_adapters : 4;
+    uint32_t ctas = 8;
+    while (ctas > 1 && (ctas / 2) * L::kCols >= a.n_cols) ctas /= 2;
+    p.cols_per_cta = ceil_div(a.n_cols, ctas * L::kCols) * L::kCols;
+    p.outs_per_cta = 2 * kPassOuts;
+    auto down = adapter_down_kernel<T, 16>;
+    if constexpr (sizeof(T) == 2)
+        if (a.n_cols % 8) down = adapter_down_kernel<T, 8>;
+    cudaError_t e = launch_cluster(down, dim3(tiles * ctas, slots), ctas, L::kBytes, a.pdl, s, p);
     if (e != cudaSuccess) return e;
     ++*launches;
-    const size_t smem = (size_t)2 * rows * ((a.max_rank + 31) / 32 * 32 + 16) * 4;
-    auto kern = rows == 8 ? adapter_up_kernel<T, 1> : adapter_up_kernel<T, 4>;
-    if (smem > 40 * 1024 && (e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
-    e = launch_kernel(kern, up, block, smem, s, true, p);
+    const size_t smem = (size_t)2 * kTileRows * v_pitch(a.max_rank) * 4;
+    auto up = adapter_up_kernel<T>;
+    if (smem > 24 * 1024 && (e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+    e = launch_kernel(up, dim3(tiles, slots, ceil_div(a.n_rows, p.outs_per_cta)), dim3(kThreads), smem, s, true, p);
     if (e == cudaSuccess) ++*launches;
     return e;
 }
 
 }  // namespace
 
-size_t adapter_scratch_bytes(const AdapterBatch &a, int sm_count) { return (size_t)a.batch * splits_of(a, sm_count) * ((a.max_rank + 3) / 4 * 4) * sizeof(float); }
+size_t adapter_scratch_bytes(const AdapterBatch &a) { return is_step(a) ? 0 : (size_t)a.batch * rank_pitch(a) * sizeof(float); }
 
-cudaError_t launch_adapters(const AdapterBatch &a, int sm_count, cudaStream_t s, uint64_t *launches) {
+cudaError_t launch_adapters(const AdapterBatch &a, cudaStream_t s, uint64_t *launches) {
     AdapterParams p = {};
     p.down = a.down, p.up = a.up, p.ranks = a.ranks, p.row_adapter = a.row_adapter, p.scales = a.scales, p.x = a.x, p.base = a.base, p.out = a.out;
     p.sums = static_cast<float *>(a.scratch);
     p.n_adapters = a.n_adapters, p.max_rank = a.max_rank, p.n_rows = a.n_rows, p.n_cols = a.n_cols, p.batch = a.batch;
     p.x_stride = a.x_stride, p.out_stride = a.out_stride;
-    p.splits = splits_of(a, sm_count);
-    p.cols_per_split = ceil_div(ceil_div(a.n_cols, p.splits), 64) * 64;
-    p.splits = ceil_div(a.n_cols, p.cols_per_split);
-    p.rank_pitch = (a.max_rank + 3) / 4 * 4;
-    p.slots = tile_rows(a) == 8 ? (a.batch < 8 ? a.batch : 8) : 1;
+    p.rank_pitch = rank_pitch(a);
     p.whole_ranks = a.max_rank % 4 == 0;
     p.whole_outs = a.n_rows % 4 == 0 && a.out_stride % 4 == 0;
-    return a.type == YULE_DTYPE_F16 ? launch_typed<__half>(a, p, s, launches) : launch_typed<float>(a, p, s, launches);
+    if (is_step(a)) return a.type == YULE_DTYPE_F16 ? launch_step<__half>(a, p, s, launches) : launch_step<float>(a, p, s, launches);
+    return a.type == YULE_DTYPE_F16 ? launch_prompts<__half>(a, p, s, launches) : launch_prompts<float>(a, p, s, launches);
 }
 
 }  // namespace yule

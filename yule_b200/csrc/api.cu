@@ -1089,10 +1089,10 @@ int32_t yule_cuda_adapter_matmul_batched(yule_cuda_ctx *ctx, yule_buffer down, y
     a.base = (const float *)B.ptr, a.out = (float *)O.ptr;
     a.type = shape->gguf_type, a.n_adapters = shape->n_adapters, a.max_rank = shape->max_rank, a.n_rows = shape->n_rows, a.n_cols = shape->n_cols, a.batch = shape->batch;
     a.x_stride = shape->x_stride, a.out_stride = shape->out_stride;
-    if (int32_t rc = ensure_batch_scratch(ctx, adapter_scratch_bytes(a, ctx->prop.multiProcessorCount))) return rc;
+    if (int32_t rc = ensure_batch_scratch(ctx, adapter_scratch_bytes(a))) return rc;
     a.scratch = ctx->batch_scratch;
     a.pdl = chain_goes_on(ctx, _chain.armed, _chain.n);
-    LAUNCHED(ctx, launch_adapters(a, ctx->prop.multiProcessorCount, ctx->stream, &_n));
+    LAUNCHED(ctx, launch_adapters(a, ctx->stream, &_n));
     chain_output(ctx, O.ptr, need.output);
     ctx->pdl_chain = true;
     return YULE_OK;
