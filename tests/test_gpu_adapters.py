@@ -153,6 +153,23 @@ def test_sizes(backend, dtype):
         c.free(backend)
 
 
+@BOTH
+@pytest.mark.parametrize("batch", [5, 77])
+def test_sizes_within_a_rank(backend, dtype, batch):
+    """Rows of `down` of very different sizes against columns of `up` that bring their products back to one size, in some adapters and some rows only."""
+    c = Call(batch=batch, dtype=dtype, rank=40, ranks=[40, 33, 40], cols=256)
+    size = (2.0 ** np.linspace(-11, 11, 40)).astype(np.float32)
+    for a in (0, 1):
+        c.down[a] = (c.down[a].astype(np.float32) * size[:, None]).astype(c.down.dtype)
+        c.up[a] = (c.up[a].astype(np.float32) / size[None]).astype(c.up.dtype)
+    c.x[::3, :] = 0
+    c.x[::3, 5] = 1
+    c.base[:] = 0
+    c.upload(backend).run(backend)
+    c.check(backend)
+    c.free(backend)
+
+
 def test_ranks_beyond_the_largest_count_as_it(backend):
     go(backend, ranks=[17, NONE, 16])
 

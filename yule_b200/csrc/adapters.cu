@@ -34,7 +34,7 @@ struct AdapterParams {
     const void *down, *up;
     const uint32_t *ranks, *row_adapter;
     const float *scales, *x, *base;
-    float *out, *sums;  // sums (prompts): [row][rank_pitch]
+    float *out, *sums, *row_scales;  // prompts: sums [row][rank_pitch], scales of rows of halves
     uint32_t n_adapters, max_rank, n_rows, n_cols, batch, cols_per_cta, outs_per_cta, rank_pitch;
     size_t x_stride, out_stride;
     bool whole_ranks, whole_outs;  // rows of `up`, and of out and base, are on the boundaries of vectors of four
@@ -69,17 +69,32 @@ __device__ __forceinline__ Slot read_slot(const Tile &t, uint32_t slot, uint8_t 
     __syncwarp();
     return {__shfl_sync(0xffffffffu, t.id, first), (uint32_t)__popc(mask)};
 }
-// Rows without an adapter: their base, outputs [o0, o1).
+// Rows without an adapter: their base, outputs [o0, o1), four of a thread's pieces under way together.
 template <uint32_t ROWS>
-__device__ __forceinline__ void copy_base(const AdapterParams &p, const Tile &t, uint32_t row0, uint32_t o0, uint32_t o1) {
-    if (p.base == p.out) return;
-    for (uint32_t none = __ballot_sync(0xffffffffu, t.id == ~0u && (threadIdx.x & 31) < ROWS && row0 + (threadIdx.x & 31) < p.batch); none; none &= none - 1) {
-        const size_t at = (size_t)(row0 + __ffs(none) - 1) * p.out_stride;
-        if (p.whole_outs)
-            for (uint32_t o = o0 + 4 * threadIdx.x; o < o1; o += 4 * kThreads) *reinterpret_cast<float4 *>(p.out + at + o) = *reinterpret_cast<const float4 *>(p.base + at + o);
-        else
-            for (uint32_t o = o0 + threadIdx.x; o < o1; o += kThreads) p.out[at + o] = p.base[at + o];
-    }
+__device__ __forceinline__ void copy_base(const AdapterParams &p, const Tile &t, uint32_t row0, uint32_t o0, uint32_t o1, uint8_t *list) {
+    const uint32_t lane = threadIdx.x & 31, mask = __ballot_sync(0xffffffffu, t.id == ~0u && lane < ROWS && row0 + lane < p.batch);
+    if (p.base == p.out || mask == 0 || o0 >= o1) return;
+    if (mask >> lane & 1u) list[__popc(mask & ((1u << lane) - 1))] = (uint8_t)lane;
+    __syncwarp();
+    auto copy = [&](auto one, uint32_t width) {
+        using V = decltype(one);
+        const uint32_t per_row = (o1 - o0) / width, n = __popc(mask) * per_row;
+        for (uint32_t i = threadIdx.x; i < n; i += 4 * kThreads) {
+            V v[4];
+            size_t at[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t e = min(i + j * kThreads, n - 1);
+                at[j] = (size_t)(row0 + list[e / per_row]) * p.out_stride + o0 + e % per_row * width;
+                v[j] = *reinterpret_cast<const V *>(p.base + at[j]);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++)
+                if (i + j * kThreads < n) *reinterpret_cast<V *>(p.out + at[j]) = v[j];
+        }
+    };
+    if (p.whole_outs) copy(float4(), 4);
+    else copy(float(), 1);
 }
 
 // Four elements of an adapter's row from `at` on, of which `n` are there, as they lie and as fp32.
@@ -164,7 +179,7 @@ template <typename T, int RANKS>
 __global__ void __launch_bounds__(kThreads, 2) adapter_step_kernel(const __grid_constant__ AdapterParams p) {
     extern __shared__ __align__(16) float got[];  // sums of v: [CTA][row][rank_pitch], then v's terms: hi, lo: [row][pitch]
     __shared__ float meet[kWarps][kStepRows][RANKS * 16 + 1];
-    __shared__ uint8_t lists[kWarps][32];
+    __shared__ uint8_t lists[kWarps][32], none_lists[kWarps][32];
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t ctas = gridDim.x, cta = blockIdx.x, row0 = blockIdx.z * kStepRows, slot_at = blockIdx.y;
@@ -174,8 +189,8 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_step_kernel(const __grid_
     yule_pdl_wait();
     const uint32_t near_rank = lane < p.n_adapters ? __ldg(p.ranks + lane) : 0u;  // (beside the rows' adapters, not behind them)
     const Tile tile = read_tile<kStepRows>(p, row0);
-    if (slot_at == 0) copy_base<kStepRows>(p, tile, row0, out0, out1);
     if (slot_at >= __popc(tile.firsts)) {  // (the same for all the cluster)
+        if (slot_at == 0) copy_base<kStepRows>(p, tile, row0, out0, out1, none_lists[warp]);
         cluster.barrier_wait(std::move(started));
         return;
     }
@@ -248,6 +263,7 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_step_kernel(const __grid_
 #pragma unroll
     for (int c = 0; c < 2; c++) at[c] = (size_t)(row0 + rows[mine[c] ? 2 * t + c : 0]) * p.out_stride, b[c] = load4(p, at[c], o, mine[c] && o < end);
     load_up(p, up, o, 0, o < end ? rank : 0, u);
+    if (slot_at == 0) copy_base<kStepRows>(p, tile, row0, out0, out1, none_lists[warp]);
     cluster.barrier_wait(std::move(summed));
     const uint32_t pitch = v_pitch(p.max_rank);
     uint32_t *v_hi = reinterpret_cast<uint32_t *>(got + ctas * kStepRows * p.rank_pitch), *v_lo = v_hi + kStepRows * pitch;
@@ -290,7 +306,8 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_step_kernel(const __grid_
 template <int W>
 __device__ __forceinline__ void copy_async(uint32_t to, const void *from, bool there) {
     const int bytes = there ? W : 0;
-    if (W == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+    if (W == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+    else if (W == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
@@ -302,6 +319,52 @@ struct DownLayout {
     static constexpr uint32_t kMeet = 4 * kTileRows * (kRanks + 1) * 4, kSum = kTileRows * kRanks * 4;
     static constexpr uint32_t kRing = kStages * kStage, kBytes = (kRing > kMeet ? kRing : kMeet) + kSum;
 };
+
+// F16 adapters of ranks to 64: a row of v as fp16 terms, v · 2^e = hi + lo up to 2^-22 of v, with its largest number in [2^14, 2^15): products of fp16 numbers at
+// twice the rate of tf32 ones.  Numbers below 2^-16 of the row's largest would lose bits of lo: a row that has such (but not zero), or one that is not finite,
+// stays as it is, with 0 as its scale.  `v`: this lane's four numbers of the row that kLanes lanes have; comes back as four hi and four lo, the inverse of 2^e in `scale`.
+template <uint32_t LANES>
+__device__ __forceinline__ float4 halves_of_row(const float4 &v, float *scale) {
+    const float all[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
+    uint32_t most = 0, least = ~0u;  // (of numbers >= 0, as their bits are ordered; NaN is above infinity)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t bits = __float_as_uint(all[i]);
+        most = max(most, bits);
+        if (bits) least = min(least, bits);
+    }
+#pragma unroll
+    for (uint32_t m = LANES / 2; m; m /= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, m)), least = min(least, __shfl_xor_sync(0xffffffffu, least, m));
+    const bool keep = most >= 0x7F800000u || (most && __uint_as_float(least) < __uint_as_float(most) * 0x1p-16f);
+    const int e = max(-113, min(126, 14 - ((int)(most >> 23) - 127)));
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+    if (scale) *scale = keep ? 0.f : __uint_as_float((uint32_t)(127 - e) << 23);
+    if (keep) return v;
+    auto terms = [&](float a, float b, uint32_t &hi, uint32_t &lo) {
+        const __half2 h = __floats2half2_rn(a * up, b * up);
+        const float2 f = __half22float2(h);
+        const __half2 l = __floats2half2_rn(a * up - f.x, b * up - f.y);
+        hi = *reinterpret_cast<const uint32_t *>(&h), lo = *reinterpret_cast<const uint32_t *>(&l);
+    };
+    uint32_t hi[2], lo[2];
+    terms(v.x, v.y, hi[0], lo[0]), terms(v.z, v.w, hi[1], lo[1]);
+    return make_float4(__uint_as_float(hi[0]), __uint_as_float(hi[1]), __uint_as_float(lo[0]), __uint_as_float(lo[1]));
+}
+__device__ __forceinline__ float4 row_of_halves(const float4 &v, float scale) {  // and back
+    auto two = [&](float hi, float lo) {
+        const uint32_t h = __float_as_uint(hi), l = __float_as_uint(lo);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h)), b = __half22float2(*reinterpret_cast<const __half2 *>(&l));
+        return make_float2((a.x + b.x) * scale, (a.y + b.y) * scale);
+    };
+    const float2 a = two(v.x, v.z), b = two(v.y, v.w);
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+// d += a · b over one step of sixteen, as for tf32: this lane's four elements of rows g (a) and g + 8 (b), and of the second operand's column g.
+__device__ __forceinline__ void multiply_f16(float (&d)[4], const uint2 &a, const uint2 &b, float v0, float v1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a.x), "r"(b.x), "r"(a.y), "r"(b.y), "r"(__float_as_uint(v0)), "r"(__float_as_uint(v1)));
+}
 
 // v of a tile's slots, 64 ranks at a time: grid x = tiles × the cluster (a share of the columns per CTA), y = slots.  A warp has 32 ranks and 16 of each 64 columns.
 template <typename T, int W>
@@ -323,28 +386,27 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_down_kernel(const __grid_
         const Slot slot = read_slot(tile, s, lists[warp]);
         const uint32_t rank = min(__ldg(p.ranks + slot.adapter), p.max_rank);
         const T *down = static_cast<const T *>(p.down) + (size_t)slot.adapter * p.max_rank * p.n_cols;
+        constexpr uint32_t kPerRow = L::kCols * sizeof(T) / W, kCopies = L::kRanks * kPerRow / kThreads;  // copies of a row of `down`, and of a thread
+        const uint32_t x_col = threadIdx.x % 16 * 4, x_row = threadIdx.x / 16, w_col = threadIdx.x % kPerRow * (W / sizeof(T)), w_row = threadIdx.x / kPerRow;
         const float *from[2];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t r = threadIdx.x / 16 + 16 * i;
-            from[i] = p.x + (size_t)(row0 + rows[r < slot.n ? r : 0]) * p.x_stride;
-        }
+        for (int i = 0; i < 2; i++) from[i] = p.x + (size_t)(row0 + rows[x_row + 16 * i < slot.n ? x_row + 16 * i : 0]) * p.x_stride + col0 + x_col;
         for (uint32_t k0 = 0; k0 < rank; k0 += L::kRanks) {
+            const T *w = down + (size_t)(k0 + w_row) * p.n_cols + col0 + w_col;
+            const size_t w_step = (size_t)(kThreads / kPerRow) * p.n_cols;
             auto load = [&](uint32_t i) {
                 if (i < n_stages) {
-                    const uint32_t stage = to + i % L::kStages * L::kStage, c0 = col0 + i * L::kCols;
+                    const uint32_t stage = to + i % L::kStages * L::kStage, c = i * L::kCols;
 #pragma unroll
                     for (int n = 0; n < 2; n++) {
-                        const uint32_t r = threadIdx.x / 16 + 16 * n, c = threadIdx.x % 16 * 4;
-                        const bool there = r < slot.n && c0 + c < col1;
-                        copy_async<16>(stage + r * L::kXPitch + c * 4, there ? from[n] + c0 + c : p.x, there);
+                        const bool there = x_row + 16 * n < slot.n && col0 + c + x_col < col1;
+                        copy_async<16>(stage + (x_row + 16 * n) * L::kXPitch + x_col * 4, there ? from[n] + c : p.x, there);
                     }
-                    constexpr uint32_t per_row = L::kCols * sizeof(T) / W;
 #pragma unroll
-                    for (uint32_t n = 0; n < L::kRanks * per_row / kThreads; n++) {
-                        const uint32_t at = threadIdx.x + n * kThreads, k = at / per_row, c = at % per_row * (W / sizeof(T));
-                        const bool there = k0 + k < rank && c0 + c < col1;
-                        copy_async<W>(stage + L::kX + k * L::kDPitch + c * sizeof(T), there ? down + (size_t)(k0 + k) * p.n_cols + c0 + c : down, there);
+                    for (uint32_t n = 0; n < kCopies; n++) {
+                        const uint32_t k = w_row + n * (kThreads / kPerRow);
+                        const bool there = k0 + k < rank && col0 + c + w_col < col1;
+                        copy_async<W>(stage + L::kX + k * L::kDPitch + w_col * sizeof(T), there ? w + n * w_step + c : down, there);
                     }
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
@@ -392,7 +454,6 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_down_kernel(const __grid_
 #pragma unroll
                     for (int e = 0; e < 4; e++) meet[(part * kTileRows + 8 * n + 2 * t + (e & 1)) * (L::kRanks + 1) + 32 * half + 16 * r + g + 8 * (e >> 1)] = sum[r][n][e];
             __syncthreads();
-            const uint32_t n_ranks = min(rank - k0, L::kRanks);
             for (uint32_t i = threadIdx.x; i < slot.n * L::kRanks; i += kThreads) {
                 const uint32_t r = i / L::kRanks, k = i % L::kRanks;
                 float v = 0.f;
@@ -401,21 +462,184 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_down_kernel(const __grid_
                 mine[i] = v;
             }
             cluster.sync();
-            for (uint32_t i = cta * kThreads + threadIdx.x; i < slot.n * L::kRanks; i += ctas * kThreads) {
-                const uint32_t r = i / L::kRanks, k = i % L::kRanks;
-                if (k >= n_ranks) continue;
-                float v = 0.f;
-                for (uint32_t c = 0; c < ctas; c++) v += cluster.map_shared_rank(mine, c)[i];
-                p.sums[(size_t)(row0 + rows[r]) * p.rank_pitch + k0 + k] = v;
+            constexpr uint32_t kLanes = L::kRanks / 4;  // of a row
+            for (uint32_t i = cta * kThreads + threadIdx.x; i < (slot.n + 1) / 2 * 2 * kLanes; i += ctas * kThreads) {  // (whole warps: two rows each)
+                const uint32_t r = i / kLanes, k = i % kLanes * 4;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < slot.n)
+                    for (uint32_t c = 0; c < ctas; c++) {
+                        const float4 of = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(mine, c) + 4 * i);
+                        v.x += of.x, v.y += of.y, v.z += of.z, v.w += of.w;
+                    }
+                if (p.row_scales) v = halves_of_row<kLanes>(v, r < slot.n && k == 0 ? p.row_scales + row0 + rows[r] : nullptr);
+                if (r < slot.n && k0 + k < p.rank_pitch) *reinterpret_cast<float4 *>(p.sums + (size_t)(row0 + rows[r]) * p.rank_pitch + k0 + k) = v;  // (beyond the rank: zeros)
             }
             cluster.sync();  // (the other CTAs have read this one's sums)
         }
+        const uint32_t done = (rank + L::kRanks - 1) / L::kRanks * L::kRanks;
+        for (uint32_t r = cta; r < slot.n; r += ctas)
+            for (uint32_t k = done + threadIdx.x; k < p.rank_pitch; k += kThreads) {
+                p.sums[(size_t)(row0 + rows[r]) * p.rank_pitch + k] = 0.f;
+                if (k == 0 && p.row_scales) p.row_scales[row0 + rows[r]] = 1.f;
+            }
     }
 }
 
-// out of a tile's slots, a share of the outputs per CTA: grid x = tiles, y = slots, z = shares.  32 outputs a warp and pass, base loaded before the products.
+// out of all rows, ranks to 64.  A CTA has 128 outputs of one tile after another (its part of all outputs of all tiles), a warp 32 of them, whose rows of `up` it keeps in
+// registers while the adapter stays the same.  Rows come in blocks of sixteen of an adapter, their base by copies into the warp's shared memory (a lane its own), their
+// v into the CTA's (a warp a fourth), both under way while the block before is worked on.
+constexpr uint32_t kUpWarps = 4, kPlaces = 3, kUpSteps = 4, kNoRow = ~0u - 1;
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) adapter_up_kernel(const __grid_constant__ AdapterParams p) {
+constexpr uint32_t kUpCtas = sizeof(T) == 2 ? 4 : 3;  // of an SM: `up` takes 32 registers, or 64
+template <typename T>
+__global__ void __launch_bounds__(kUpWarps * 32, kUpCtas<T>) adapter_up_kernel(const __grid_constant__ AdapterParams p) {
+    struct Block {
+        uint32_t n, adapter, out0, fresh;  // fresh: other rows of `up` than the block before
+        uint32_t row[16];
+        float row_scale[16];
+    };
+    extern __shared__ __align__(16) float4 copies[];  // [place][warp][base of four rows][lane], then [place][pieces of v: of two rows per step][lane]
+    __shared__ Block blocks[kUpWarps][kPlaces];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, steps = p.rank_pitch / 16;
+    float4 *bases = copies + warp * 4 * 32 + lane, *vs = copies + kPlaces * kUpWarps * 4 * 32 + lane;
+    yule_pdl_launch_dependents();
+    yule_pdl_wait();
+    const uint32_t tiles = (p.batch - 1) / kTileRows + 1;
+    const uint64_t items = (uint64_t)tiles * ((p.n_rows + kUpWarps * 32 - 1) / (kUpWarps * 32)), begin = blockIdx.x * items / gridDim.x;
+    uint32_t left = (uint32_t)((blockIdx.x + 1) * items / gridDim.x - begin), tile = (uint32_t)(begin % tiles), out0 = ((uint32_t)(begin / tiles) * kUpWarps + warp) * 32;
+    uint32_t firsts = 0, rows = 0, adapter = 0, id = 0, row0 = 0, fresh = 0;
+    auto read_id = [&](uint32_t of) { return of * kTileRows + lane < p.batch ? __ldg(p.row_adapter + of * kTileRows + lane) : 0u; };  // (looked at a tile later: nothing waits for it here)
+    uint32_t id_next = left ? read_id(tile) : 0u, adapter_before = kNoRow, out_before = 0;
+    // The next block, its copies under way (an empty group behind the last one).
+    auto fetch = [&](uint32_t place) {
+        Block &block = blocks[warp][place];
+        while (rows == 0) {
+            while (firsts == 0 && left) {
+                left--, row0 = tile * kTileRows, id = row0 + lane >= p.batch ? kNoRow : id_next < p.n_adapters ? id_next : ~0u;
+                const uint32_t same = __match_any_sync(0xffffffffu, id);
+                // (rows without an adapter are blocks like the others where there is something to copy)
+                firsts = __ballot_sync(0xffffffffu, (uint32_t)__ffs(same) == lane + 1 && id != kNoRow && (id != ~0u || p.base != p.out));
+                fresh = out0;
+                if (++tile == tiles) tile = 0, out0 += kUpWarps * 32;
+                if (left) id_next = read_id(tile);
+            }
+            if (firsts == 0) break;
+            adapter = __shfl_sync(0xffffffffu, id, __ffs(firsts) - 1);
+            firsts &= firsts - 1;
+            rows = __ballot_sync(0xffffffffu, id == adapter);
+        }
+        const uint32_t before = __popc(rows & ((1u << lane) - 1)), n = min((uint32_t)__popc(rows), 16u), o = fresh + 4 * g;
+        const bool taken = (rows >> lane & 1u) && before < 16;
+        __syncwarp();  // (the block that was here has been read)
+        if (taken) {
+            block.row[before] = row0 + lane;
+            if (sizeof(T) == 2 && adapter != ~0u) copy_async<4>((uint32_t)__cvta_generic_to_shared(block.row_scale + before), p.row_scales + row0 + lane, true);
+        }
+        if (lane == 0) block.n = n, block.adapter = adapter, block.out0 = fresh, block.fresh = adapter != adapter_before || fresh != out_before;
+        adapter_before = adapter, out_before = fresh;
+        rows &= ~__ballot_sync(0xffffffffu, taken);
+        __syncwarp();
+        if (n) {
+            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(bases + place * kUpWarps * 4 * 32), v_dst = (uint32_t)__cvta_generic_to_shared(vs + place * 2 * steps * 32);
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) {
+                const uint32_t r = c / 2 * 8 + 2 * t + c % 2;
+                if (r >= n) continue;
+                const float *from = p.base + (size_t)block.row[r] * p.out_stride + o;
+                if (p.whole_outs) {
+                    if (o < p.n_rows) copy_async<16>(dst + c * 512, from, true);
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++)
+                        if (o + i < p.n_rows) copy_async<4>(dst + c * 512 + 4 * i, from + i, true);
+                }
+            }
+            if (adapter != ~0u) {
+                const uint32_t half = warp & 1u, r = g + 8 * half;  // pieces warp and warp + 4: steps warp / 2 and warp / 2 + 2 of rows r
+                const float *v = p.sums + (size_t)block.row[r < n ? r : 0] * p.rank_pitch + 4 * t;
+                if (8 * half < n)
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; i++) {
+                        const uint32_t j = warp / 2 + 2 * i;
+                        if (j < steps) copy_async<16>(v_dst + (2 * j + half) * 512, v + 16 * j, true);
+                    }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    static_assert(kUpWarps == 4 && kUpSteps == 4, "who copies what of v");
+    uint32_t place = 0, ahead = 0;
+    float scale = 0.f;
+    Four<T> up[kUpSteps][4];
+    fetch(ahead++);
+    for (;;) {
+        fetch(ahead);  // (where the block before the last one was: all have been here since)
+        ahead = ahead == kPlaces - 1 ? 0 : ahead + 1;
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncthreads();
+        const Block &block = blocks[warp][place];
+        const uint32_t n = block.n, of = block.adapter, o = block.out0 + 4 * g;
+        if (n == 0) return;
+        scale = of == ~0u ? -0.f : scale;  // (-0 · 0 + base: its bits)
+        if (block.fresh && of != ~0u) {
+            const uint32_t rank = min(__ldg(p.ranks + of), p.max_rank);
+            scale = __ldg(p.scales + of);
+            const T *first = static_cast<const T *>(p.up) + (size_t)of * p.n_rows * p.max_rank;
+#pragma unroll
+            for (uint32_t j = 0; j < kUpSteps; j++) load_up(p, first, o, j, rank, up[j]);
+        }
+        const float4 *from = bases + place * kUpWarps * 4 * 32, *v = vs + place * 2 * steps * 32;
+        float d[2][2][4] = {};
+        bool halves = false;
+        if constexpr (sizeof(T) == 2) {
+            const float mine = block.row_scale[lane & 15];
+            halves = !__any_sync(0xffffffffu, (lane & 15) < n && mine == 0.f) && of != ~0u;
+            if (halves)
+#pragma unroll
+                for (uint32_t j = 0; j < kUpSteps; j++) {
+                    if (j == steps) break;
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; h++) {
+                        const float4 w = v[(2 * j + h) * 32];
+                        multiply_f16(d[h][0], up[j][0].v, up[j][1].v, w.z, w.w);
+                        multiply_f16(d[h][1], up[j][2].v, up[j][3].v, w.z, w.w);
+                        multiply_f16(d[h][0], up[j][0].v, up[j][1].v, w.x, w.y);
+                        multiply_f16(d[h][1], up[j][2].v, up[j][3].v, w.x, w.y);
+                    }
+                }
+        }
+        if (!halves && of != ~0u)
+#pragma unroll
+            for (uint32_t j = 0; j < kUpSteps; j++) {
+                if (j == steps) break;
+                float4 a[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) a[i] = up[j][i].get();
+#pragma unroll
+                for (uint32_t h = 0; h < 2; h++) {
+                    float4 w = v[(2 * j + h) * 32];
+                    if (sizeof(T) == 2 && g + 8 * h < n && block.row_scale[g + 8 * h] != 0.f) w = row_of_halves(w, block.row_scale[g + 8 * h]);
+                    uint4 hi, lo;
+                    split4(w, hi, lo);
+                    multiply<sizeof(T) == 2>(d[h][0], a[0], a[1], hi, lo);
+                    multiply<sizeof(T) == 2>(d[h][1], a[2], a[3], hi, lo);
+                }
+            }
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++) {
+            const uint32_t r = c / 2 * 8 + 2 * t + c % 2;
+            const float(&e)[2][4] = d[c / 2];
+            const float back = halves ? block.row_scale[r] : 1.f;
+            const float four_of[4] = {e[0][c % 2] * back, e[0][2 + c % 2] * back, e[1][c % 2] * back, e[1][2 + c % 2] * back};
+            if (r < n) store4(p, (size_t)block.row[r] * p.out_stride, o, from[c * 32], four_of, scale);
+        }
+        place = place == kPlaces - 1 ? 0 : place + 1;
+    }
+}
+
+// out of a tile's slots, larger ranks, a share of the outputs per CTA: grid x = tiles, y = slots, z = shares.  32 outputs a warp and pass.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) adapter_up_wide_kernel(const __grid_constant__ AdapterParams p) {
     extern __shared__ __align__(16) uint32_t v_hi[];  // hi, then lo: [row][pitch]
     __shared__ uint8_t lists[kWarps][32];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -424,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_up_kernel(const __grid_co
     yule_pdl_launch_dependents();
     yule_pdl_wait();
     const Tile tile = read_tile<kTileRows>(p, row0);
-    if (blockIdx.y == 0) copy_base<kTileRows>(p, tile, row0, out0, end);
+    if (blockIdx.y == 0) copy_base<kTileRows>(p, tile, row0, out0, end, lists[warp]);
     const uint32_t n_slots = __popc(tile.firsts);
     const uint8_t *rows = lists[warp];
     for (uint32_t s = blockIdx.y; s < n_slots; s += gridDim.y) {
@@ -474,8 +698,8 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_up_kernel(const __grid_co
 }
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
-uint32_t rank_pitch(const AdapterBatch &a) { return (a.max_rank + 3) / 4 * 4; }
 bool is_step(const AdapterBatch &a) { return a.batch <= 64; }
+uint32_t rank_pitch(const AdapterBatch &a) { return is_step(a) ? (a.max_rank + 3) / 4 * 4 : (a.max_rank + 15) / 16 * 16; }
 
 cudaError_t launch_cluster(void (*kern)(AdapterParams), dim3 grid, uint32_t ctas, size_t smem, bool pdl, cudaStream_t s, const AdapterParams &p) {
     cudaError_t e;
@@ -508,42 +732,51 @@ cudaError_t launch_step(const AdapterBatch &a, AdapterParams p, cudaStream_t s, 
 }
 
 template <typename T>
-cudaError_t launch_prompts(const AdapterBatch &a, AdapterParams p, cudaStream_t s, uint64_t *launches) {
+cudaError_t launch_prompts(const AdapterBatch &a, AdapterParams p, int sm_count, cudaStream_t s, uint64_t *launches) {
     using L = DownLayout<T>;
     const uint32_t tiles = ceil_div(a.batch, kTileRows), slots = a.n_adapters < 4 ? a.n_adapters : 4;
     uint32_t ctas = 8;
-    while (ctas > 1 && (ctas / 2) * L::kCols >= a.n_cols) ctas /= 2;
+    while (ctas > 1 && ((ctas - 1) * L::kCols >= a.n_cols || (uint64_t)tiles * ctas > 7 * (uint64_t)sm_count / 4)) ctas--;
     p.cols_per_cta = ceil_div(a.n_cols, ctas * L::kCols) * L::kCols;
-    p.outs_per_cta = 2 * kPassOuts;
     auto down = adapter_down_kernel<T, 16>;
     if constexpr (sizeof(T) == 2)
         if (a.n_cols % 8) down = adapter_down_kernel<T, 8>;
     cudaError_t e = launch_cluster(down, dim3(tiles * ctas, slots), ctas, L::kBytes, a.pdl, s, p);
     if (e != cudaSuccess) return e;
     ++*launches;
-    const size_t smem = (size_t)2 * kTileRows * v_pitch(a.max_rank) * 4;
-    auto up = adapter_up_kernel<T>;
-    if (smem > 24 * 1024 && (e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
-    e = launch_kernel(up, dim3(tiles, slots, ceil_div(a.n_rows, p.outs_per_cta)), dim3(kThreads), smem, s, true, p);
+    if (a.max_rank <= 16 * kUpSteps) {
+        const uint64_t items = (uint64_t)tiles * ceil_div(a.n_rows, kUpWarps * 32), at_once = kUpCtas<T> * (uint64_t)sm_count;
+        const size_t smem = (size_t)kPlaces * (kUpWarps * 4 + p.rank_pitch / 8) * 512;
+        auto up = adapter_up_kernel<T>;
+        if ((e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+        e = launch_kernel(up, dim3((uint32_t)(items < at_once ? items : at_once)), dim3(kUpWarps * 32), smem, s, true, p);
+    } else {
+        p.outs_per_cta = 2 * kPassOuts;
+        const size_t smem = (size_t)2 * kTileRows * v_pitch(a.max_rank) * 4;
+        auto up = adapter_up_wide_kernel<T>;
+        if ((e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+        e = launch_kernel(up, dim3(tiles, slots, ceil_div(a.n_rows, p.outs_per_cta)), dim3(kThreads), smem, s, true, p);
+    }
     if (e == cudaSuccess) ++*launches;
     return e;
 }
 
 }  // namespace
 
-size_t adapter_scratch_bytes(const AdapterBatch &a) { return is_step(a) ? 0 : (size_t)a.batch * rank_pitch(a) * sizeof(float); }
+size_t adapter_scratch_bytes(const AdapterBatch &a) { return is_step(a) ? 0 : (size_t)a.batch * (rank_pitch(a) + 1) * sizeof(float); }
 
-cudaError_t launch_adapters(const AdapterBatch &a, cudaStream_t s, uint64_t *launches) {
+cudaError_t launch_adapters(const AdapterBatch &a, int sm_count, cudaStream_t s, uint64_t *launches) {
     AdapterParams p = {};
     p.down = a.down, p.up = a.up, p.ranks = a.ranks, p.row_adapter = a.row_adapter, p.scales = a.scales, p.x = a.x, p.base = a.base, p.out = a.out;
     p.sums = static_cast<float *>(a.scratch);
     p.n_adapters = a.n_adapters, p.max_rank = a.max_rank, p.n_rows = a.n_rows, p.n_cols = a.n_cols, p.batch = a.batch;
     p.x_stride = a.x_stride, p.out_stride = a.out_stride;
     p.rank_pitch = rank_pitch(a);
+    p.row_scales = a.type == YULE_DTYPE_F16 && a.max_rank <= 16 * kUpSteps ? p.sums + (size_t)a.batch * p.rank_pitch : nullptr;
     p.whole_ranks = a.max_rank % 4 == 0;
     p.whole_outs = a.n_rows % 4 == 0 && a.out_stride % 4 == 0;
     if (is_step(a)) return a.type == YULE_DTYPE_F16 ? launch_step<__half>(a, p, s, launches) : launch_step<float>(a, p, s, launches);
-    return a.type == YULE_DTYPE_F16 ? launch_prompts<__half>(a, p, s, launches) : launch_prompts<float>(a, p, s, launches);
+    return a.type == YULE_DTYPE_F16 ? launch_prompts<__half>(a, p, sm_count, s, launches) : launch_prompts<float>(a, p, sm_count, s, launches);
 }
 
 }  // namespace yule

@@ -1092,7 +1092,7 @@ int32_t yule_cuda_adapter_matmul_batched(yule_cuda_ctx *ctx, yule_buffer down, y
     if (int32_t rc = ensure_batch_scratch(ctx, adapter_scratch_bytes(a))) return rc;
     a.scratch = ctx->batch_scratch;
     a.pdl = chain_goes_on(ctx, _chain.armed, _chain.n);
-    LAUNCHED(ctx, launch_adapters(a, ctx->stream, &_n));
+    LAUNCHED(ctx, launch_adapters(a, ctx->prop.multiProcessorCount, ctx->stream, &_n));
     chain_output(ctx, O.ptr, need.output);
     ctx->pdl_chain = true;
     return YULE_OK;

@@ -578,7 +578,7 @@ struct AdapterBatch {
     bool pdl = false;
 };
 size_t adapter_scratch_bytes(const AdapterBatch &a);
-cudaError_t launch_adapters(const AdapterBatch &a, cudaStream_t s, uint64_t *launches);
+cudaError_t launch_adapters(const AdapterBatch &a, int sm_count, cudaStream_t s, uint64_t *launches);
 // Verification of drafted tokens (verify.cu): the members are those of yule_verification; draft null: drafts without probabilities, lens null: n_draft each.
 struct VerifyDrafts {
     const float *target = nullptr, *draft = nullptr;
