@@ -486,99 +486,113 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_down_kernel(const __grid_
 }
 
 // out of all rows, ranks to 64.  A CTA has 128 outputs of one tile after another (its part of all outputs of all tiles), a warp 32 of them, whose rows of `up` it keeps in
-// registers while the adapter stays the same.  Rows come in blocks of sixteen of an adapter, their base by copies into the warp's shared memory (a lane its own), their
-// v into the CTA's (a warp a fourth), both under way while the block before is worked on.
-constexpr uint32_t kUpWarps = 4, kPlaces = 3, kUpSteps = 4, kNoRow = ~0u - 1;
+// registers while the adapter stays the same.  Rows come in blocks of sixteen of an adapter.  A fifth warp finds them and has their base
+// and v copied into shared memory two blocks ahead; named barriers hand the places over and back.
+constexpr uint32_t kUpWarps = 4, kPlaces = 4, kAhead = 2, kUpSteps = 4, kNoRow = ~0u - 1, kUpThreads = (kUpWarps + 1) * 32;
+__device__ __forceinline__ void barrier_sync(uint32_t id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kUpThreads) : "memory"); }
+__device__ __forceinline__ void barrier_arrive(uint32_t id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kUpThreads) : "memory"); }
 template <typename T>
 constexpr uint32_t kUpCtas = sizeof(T) == 2 ? 4 : 3;  // of an SM: `up` takes 32 registers, or 64
 template <typename T>
-__global__ void __launch_bounds__(kUpWarps * 32, kUpCtas<T>) adapter_up_kernel(const __grid_constant__ AdapterParams p) {
+__global__ void __launch_bounds__(kUpThreads, kUpCtas<T>) adapter_up_kernel(const __grid_constant__ AdapterParams p) {
     struct Block {
         uint32_t n, adapter, out0, fresh;  // fresh: other rows of `up` than the block before
         uint32_t row[16];
         float row_scale[16];
     };
     extern __shared__ __align__(16) float4 copies[];  // [place][warp][base of four rows][lane], then [place][pieces of v: of two rows per step][lane]
-    __shared__ Block blocks[kUpWarps][kPlaces];
+    __shared__ Block blocks[kPlaces];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, steps = p.rank_pitch / 16;
-    float4 *bases = copies + warp * 4 * 32 + lane, *vs = copies + kPlaces * kUpWarps * 4 * 32 + lane;
+    float4 *bases = copies + lane, *vs = copies + kPlaces * kUpWarps * 4 * 32 + lane;
+    constexpr uint32_t kFull = 1, kEmpty = 1 + kPlaces;  // barriers of the places
     yule_pdl_launch_dependents();
     yule_pdl_wait();
-    const uint32_t tiles = (p.batch - 1) / kTileRows + 1;
-    const uint64_t items = (uint64_t)tiles * ((p.n_rows + kUpWarps * 32 - 1) / (kUpWarps * 32)), begin = blockIdx.x * items / gridDim.x;
-    uint32_t left = (uint32_t)((blockIdx.x + 1) * items / gridDim.x - begin), tile = (uint32_t)(begin % tiles), out0 = ((uint32_t)(begin / tiles) * kUpWarps + warp) * 32;
-    uint32_t firsts = 0, rows = 0, adapter = 0, id = 0, row0 = 0, fresh = 0;
-    auto read_id = [&](uint32_t of) { return of * kTileRows + lane < p.batch ? __ldg(p.row_adapter + of * kTileRows + lane) : 0u; };  // (looked at a tile later: nothing waits for it here)
-    uint32_t id_next = left ? read_id(tile) : 0u, adapter_before = kNoRow, out_before = 0;
-    // The next block, its copies under way (an empty group behind the last one).
-    auto fetch = [&](uint32_t place) {
-        Block &block = blocks[warp][place];
-        while (rows == 0) {
-            while (firsts == 0 && left) {
-                left--, row0 = tile * kTileRows, id = row0 + lane >= p.batch ? kNoRow : id_next < p.n_adapters ? id_next : ~0u;
-                const uint32_t same = __match_any_sync(0xffffffffu, id);
-                // (rows without an adapter are blocks like the others where there is something to copy)
-                firsts = __ballot_sync(0xffffffffu, (uint32_t)__ffs(same) == lane + 1 && id != kNoRow && (id != ~0u || p.base != p.out));
-                fresh = out0;
-                if (++tile == tiles) tile = 0, out0 += kUpWarps * 32;
-                if (left) id_next = read_id(tile);
+    if (warp == kUpWarps) {
+        const uint32_t tiles = (p.batch - 1) / kTileRows + 1;
+        const uint64_t items = (uint64_t)tiles * ((p.n_rows + kUpWarps * 32 - 1) / (kUpWarps * 32)), begin = blockIdx.x * items / gridDim.x;
+        uint32_t left = (uint32_t)((blockIdx.x + 1) * items / gridDim.x - begin), tile = (uint32_t)(begin % tiles), out0 = (uint32_t)(begin / tiles) * kUpWarps * 32;
+        uint32_t firsts = 0, rows = 0, adapter = 0, id = 0, row0 = 0, fresh = 0;
+        auto read_id = [&](uint32_t of) { return of * kTileRows + lane < p.batch ? __ldg(p.row_adapter + of * kTileRows + lane) : 0u; };  // (looked at a tile later: nothing waits for it here)
+        uint32_t id_next = left ? read_id(tile) : 0u, adapter_before = kNoRow, out_before = 0;
+        // The next block, its copies under way (an empty group behind the last one).
+        auto fetch = [&](uint32_t place) {
+            Block &block = blocks[place];
+            while (rows == 0) {
+                while (firsts == 0 && left) {
+                    left--, row0 = tile * kTileRows, id = row0 + lane >= p.batch ? kNoRow : id_next < p.n_adapters ? id_next : ~0u;
+                    const uint32_t same = __match_any_sync(0xffffffffu, id);
+                    // (rows without an adapter are blocks like the others where there is something to copy)
+                    firsts = __ballot_sync(0xffffffffu, (uint32_t)__ffs(same) == lane + 1 && id != kNoRow && (id != ~0u || p.base != p.out));
+                    fresh = out0;
+                    if (++tile == tiles) tile = 0, out0 += kUpWarps * 32;
+                    if (left) id_next = read_id(tile);
+                }
+                if (firsts == 0) break;
+                adapter = __shfl_sync(0xffffffffu, id, __ffs(firsts) - 1);
+                firsts &= firsts - 1;
+                rows = __ballot_sync(0xffffffffu, id == adapter);
             }
-            if (firsts == 0) break;
-            adapter = __shfl_sync(0xffffffffu, id, __ffs(firsts) - 1);
-            firsts &= firsts - 1;
-            rows = __ballot_sync(0xffffffffu, id == adapter);
-        }
-        const uint32_t before = __popc(rows & ((1u << lane) - 1)), n = min((uint32_t)__popc(rows), 16u), o = fresh + 4 * g;
-        const bool taken = (rows >> lane & 1u) && before < 16;
-        __syncwarp();  // (the block that was here has been read)
-        if (taken) {
-            block.row[before] = row0 + lane;
-            if (sizeof(T) == 2 && adapter != ~0u) copy_async<4>((uint32_t)__cvta_generic_to_shared(block.row_scale + before), p.row_scales + row0 + lane, true);
-        }
-        if (lane == 0) block.n = n, block.adapter = adapter, block.out0 = fresh, block.fresh = adapter != adapter_before || fresh != out_before;
-        adapter_before = adapter, out_before = fresh;
-        rows &= ~__ballot_sync(0xffffffffu, taken);
-        __syncwarp();
-        if (n) {
-            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(bases + place * kUpWarps * 4 * 32), v_dst = (uint32_t)__cvta_generic_to_shared(vs + place * 2 * steps * 32);
+            const uint32_t before = __popc(rows & ((1u << lane) - 1)), n = min((uint32_t)__popc(rows), 16u), o = fresh + 4 * g;
+            const bool taken = (rows >> lane & 1u) && before < 16;
+            if (taken) {
+                block.row[before] = row0 + lane;
+                if (sizeof(T) == 2 && adapter != ~0u) copy_async<4>((uint32_t)__cvta_generic_to_shared(block.row_scale + before), p.row_scales + row0 + lane, true);
+            }
+            if (lane == 0) block.n = n, block.adapter = adapter, block.out0 = fresh, block.fresh = adapter != adapter_before || fresh != out_before;
+            adapter_before = adapter, out_before = fresh;
+            rows &= ~__ballot_sync(0xffffffffu, taken);
+            __syncwarp();
+            if (n) {
+                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(bases + place * kUpWarps * 4 * 32), v_dst = (uint32_t)__cvta_generic_to_shared(vs + place * 2 * steps * 32);
+                if (adapter != ~0u)
 #pragma unroll
-            for (uint32_t c = 0; c < 4; c++) {
-                const uint32_t r = c / 2 * 8 + 2 * t + c % 2;
-                if (r >= n) continue;
-                const float *from = p.base + (size_t)block.row[r] * p.out_stride + o;
-                if (p.whole_outs) {
-                    if (o < p.n_rows) copy_async<16>(dst + c * 512, from, true);
-                } else {
+                    for (uint32_t h = 0; h < 2; h++) {
+                        if (8 * h >= n) break;
+                        const float *v = p.sums + (size_t)block.row[g + 8 * h < n ? g + 8 * h : 0] * p.rank_pitch + 4 * t;
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; i++)
-                        if (o + i < p.n_rows) copy_async<4>(dst + c * 512 + 4 * i, from + i, true);
+                        for (uint32_t j = 0; j < kUpSteps; j++)
+                            if (j < steps) copy_async<16>(v_dst + (2 * j + h) * 512, v + 16 * j, true);
+                    }
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++) {
+                    const uint32_t r = c / 2 * 8 + 2 * t + c % 2;
+                    if (r >= n) continue;
+                    const float *from = p.base + (size_t)block.row[r] * p.out_stride + o;
+#pragma unroll
+                    for (uint32_t w = 0; w < kUpWarps; w++)
+                        if (p.whole_outs) {
+                            if (o + 32 * w < p.n_rows) copy_async<16>(dst + (4 * w + c) * 512, from + 32 * w, true);
+                        } else {
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; i++)
+                                if (o + 32 * w + i < p.n_rows) copy_async<4>(dst + (4 * w + c) * 512 + 4 * i, from + 32 * w + i, true);
+                        }
                 }
             }
-            if (adapter != ~0u) {
-                const uint32_t half = warp & 1u, r = g + 8 * half;  // pieces warp and warp + 4: steps warp / 2 and warp / 2 + 2 of rows r
-                const float *v = p.sums + (size_t)block.row[r < n ? r : 0] * p.rank_pitch + 4 * t;
-                if (8 * half < n)
-#pragma unroll
-                    for (uint32_t i = 0; i < 2; i++) {
-                        const uint32_t j = warp / 2 + 2 * i;
-                        if (j < steps) copy_async<16>(v_dst + (2 * j + half) * 512, v + 16 * j, true);
-                    }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            return n != 0;
+        };
+        uint32_t place = 0, of = 0;  // of the next block, and how many have been fetched
+        for (bool more = true; more; of++) {
+            if (of >= kPlaces) barrier_sync(kEmpty + place);
+            more = fetch(place);
+            if (of >= kAhead) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+                barrier_arrive(kFull + (place + kPlaces - kAhead) % kPlaces);
             }
+            place = place == kPlaces - 1 ? 0 : place + 1;
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    static_assert(kUpWarps == 4 && kUpSteps == 4, "who copies what of v");
-    uint32_t place = 0, ahead = 0;
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        for (uint32_t i = of < kAhead ? of : kAhead; i; i--) barrier_arrive(kFull + (place + kPlaces - i) % kPlaces);
+        return;
+    }
+    uint32_t place = 0;
     float scale = 0.f;
     Four<T> up[kUpSteps][4];
-    fetch(ahead++);
     for (;;) {
-        fetch(ahead);  // (where the block before the last one was: all have been here since)
-        ahead = ahead == kPlaces - 1 ? 0 : ahead + 1;
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        __syncthreads();
-        const Block &block = blocks[warp][place];
-        const uint32_t n = block.n, of = block.adapter, o = block.out0 + 4 * g;
+        barrier_sync(kFull + place);
+        const Block &block = blocks[place];
+        const uint32_t n = block.n, of = block.adapter, o = block.out0 + 32 * warp + 4 * g;
         if (n == 0) return;
         scale = of == ~0u ? -0.f : scale;  // (-0 · 0 + base: its bits)
         if (block.fresh && of != ~0u) {
@@ -588,7 +602,7 @@ __global__ void __launch_bounds__(kUpWarps * 32, kUpCtas<T>) adapter_up_kernel(c
 #pragma unroll
             for (uint32_t j = 0; j < kUpSteps; j++) load_up(p, first, o, j, rank, up[j]);
         }
-        const float4 *from = bases + place * kUpWarps * 4 * 32, *v = vs + place * 2 * steps * 32;
+        const float4 *from = bases + (place * kUpWarps + warp) * 4 * 32, *v = vs + place * 2 * steps * 32;
         float d[2][2][4] = {};
         bool halves = false;
         if constexpr (sizeof(T) == 2) {
@@ -633,6 +647,7 @@ __global__ void __launch_bounds__(kUpWarps * 32, kUpCtas<T>) adapter_up_kernel(c
             const float four_of[4] = {e[0][c % 2] * back, e[0][2 + c % 2] * back, e[1][c % 2] * back, e[1][2 + c % 2] * back};
             if (r < n) store4(p, (size_t)block.row[r] * p.out_stride, o, from[c * 32], four_of, scale);
         }
+        barrier_arrive(kEmpty + place);
         place = place == kPlaces - 1 ? 0 : place + 1;
     }
 }
@@ -749,7 +764,7 @@ cudaError_t launch_prompts(const AdapterBatch &a, AdapterParams p, int sm_count,
         const size_t smem = (size_t)kPlaces * (kUpWarps * 4 + p.rank_pitch / 8) * 512;
         auto up = adapter_up_kernel<T>;
         if ((e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
-        e = launch_kernel(up, dim3((uint32_t)(items < at_once ? items : at_once)), dim3(kUpWarps * 32), smem, s, true, p);
+        e = launch_kernel(up, dim3((uint32_t)(items < at_once ? items : at_once)), dim3(kUpThreads), smem, s, true, p);
     } else {
         p.outs_per_cta = 2 * kPassOuts;
         const size_t smem = (size_t)2 * kTileRows * v_pitch(a.max_rank) * 4;
