@@ -82,24 +82,24 @@ BOTH = pytest.mark.parametrize("dtype", [DType.F16, DType.F32])
 @pytest.mark.parametrize("rank", [1, 3, 4, 7, 8, 12, 16, 17, 32, 50, 64, 65, 128, 256])
 def test_ranks(backend, dtype, rank):
     go(backend, dtype=dtype, rank=rank, seed=rank)
-    go(backend, dtype=dtype, rank=rank, batch=70, rows=33, seed=rank, ranks=[rank, max(1, rank - 1), (rank + 1) // 2])
+    go(backend, dtype=dtype, rank=rank, batch=134, rows=33, seed=rank, ranks=[rank, max(1, rank - 1), (rank + 1) // 2])
 
 
 @BOTH
 @pytest.mark.parametrize("rows,cols", [(1, 4), (3, 8), (31, 12), (32, 60), (33, 64), (128, 68), (129, 256), (130, 260), (1000, 2560), (2048, 5632)])
 def test_projections(backend, dtype, rows, cols):
     go(backend, dtype=dtype, rows=rows, cols=cols, seed=rows)
-    go(backend, dtype=dtype, rows=rows, cols=cols, batch=65, seed=rows)
+    go(backend, dtype=dtype, rows=rows, cols=cols, batch=129, seed=rows)
 
 
 @BOTH
-@pytest.mark.parametrize("batch", [1, 2, 7, 8, 9, 31, 32, 33, 64, 65, 95, 96, 97, 200, 257])
+@pytest.mark.parametrize("batch", [1, 2, 7, 8, 9, 31, 32, 33, 64, 65, 127, 128, 129, 159, 160, 161, 257])
 def test_batches(backend, dtype, batch):
     go(backend, dtype=dtype, batch=batch, adapters=40, seed=batch)
     go(backend, dtype=dtype, batch=batch, adapters=2, seed=batch, in_place=True)
 
 
-@pytest.mark.parametrize("batch", [6, 100])
+@pytest.mark.parametrize("batch", [6, 164])
 def test_order_of_the_rows_does_not_matter(backend, batch):
     """Neighbours of one adapter, all of one, all different, none at all."""
     for ids in (np.zeros(batch), np.arange(batch) % 50, np.full(batch, NONE), np.arange(batch) // 3, np.where(np.arange(batch) % 2, 49, 50), (np.arange(batch) * 7) % 51):
@@ -107,7 +107,7 @@ def test_order_of_the_rows_does_not_matter(backend, batch):
         go(backend, batch=batch, adapters=50, ids=ids, in_place=True)
 
 
-@pytest.mark.parametrize("batch", [5, 77])
+@pytest.mark.parametrize("batch", [5, 141])
 def test_strides(backend, batch):
     """Rows of x, base and output further apart than they are long (vectors of four or not), NaN and marks between them."""
     for pad_out in (0, 1, 4, 6):
@@ -116,7 +116,7 @@ def test_strides(backend, batch):
 
 
 @BOTH
-@pytest.mark.parametrize("batch", [5, 77])
+@pytest.mark.parametrize("batch", [5, 141])
 def test_what_lies_beyond_a_rank_does_not_count(backend, dtype, batch):
     for rank in (16, 18):
         c = Call(batch=batch, dtype=dtype, rank=rank, ranks=[0, 5, 14], adapters=3)
@@ -127,7 +127,7 @@ def test_what_lies_beyond_a_rank_does_not_count(backend, dtype, batch):
         c.free(backend)
 
 
-@pytest.mark.parametrize("batch", [5, 77])
+@pytest.mark.parametrize("batch", [5, 141])
 def test_a_row_that_is_not_finite_stays_by_itself(backend, batch):
     c = Call(batch=batch, ids=np.arange(batch) % 3, ranks=[16, 16, 16])
     clean = c.reference()
@@ -143,7 +143,7 @@ def test_a_row_that_is_not_finite_stays_by_itself(backend, batch):
 @BOTH
 def test_sizes(backend, dtype):
     """Inputs of very different sizes in one batch, and within a row."""
-    for batch in (5, 77):
+    for batch in (5, 141):
         c = Call(batch=batch, dtype=dtype, cols=512)
         c.x *= (10.0 ** np.linspace(-25, 25, batch)).astype(np.float32)[:, None]
         c.x[:, ::3] *= np.float32(2.0 ** -12)
@@ -154,7 +154,7 @@ def test_sizes(backend, dtype):
 
 
 @BOTH
-@pytest.mark.parametrize("batch", [5, 77])
+@pytest.mark.parametrize("batch", [5, 141])
 def test_sizes_within_a_rank(backend, dtype, batch):
     """Rows of `down` of very different sizes against columns of `up` that bring their products back to one size, in some adapters and some rows only."""
     c = Call(batch=batch, dtype=dtype, rank=40, ranks=[40, 33, 40], cols=256)
@@ -175,7 +175,7 @@ def test_ranks_beyond_the_largest_count_as_it(backend):
 
 
 def test_same_bits_again(backend):
-    for batch in (9, 150):
+    for batch in (9, 214):
         c = Call(batch=batch, rows=500, cols=1024).upload(backend)
         c.run(backend)
         first = c.got(backend)
@@ -247,7 +247,7 @@ def test_refusals(backend):
 
 def test_a_capture_cannot_grow_the_scratch():
     b = CudaB200Backend(0)
-    c = Call(batch=70).upload(b)
+    c = Call(batch=134).upload(b)
     b.graph_begin()
     with pytest.raises(YuleGpuError, match="outside the capture"):
         c.run(b)

@@ -6,11 +6,14 @@
 // so an adapter is read once per tile whatever the order of the requests.  F16 adapters are tf32 numbers as they are: two products per element (with hi and lo of
 // x or v), three for F32 ones.  Sums are added in a fixed order.
 //
-// Decode steps (to 64 rows, tiles of 8): one launch, a cluster of CTAs per slot.  What there is to read is an adapter's 0.1 to 2 MB, so time goes by in latency:
-// a CTA takes a share of the columns for all ranks, writes its sums into every other CTA's shared memory, and has its share of the outputs, whose first rows of `up` and
-// of base it loads before the barrier.
-// Prompts (tiles of 32): two launches, since base and output are most of the traffic and want CTAs of their own; the first as above, the sums joined over a
-// cluster's shared memory into the scratch.
+// Decode steps (tiles of 8): one launch, a cluster of CTAs per slot.  What there is to read is an adapter's 0.1 to 2 MB, so time goes by in latency: a CTA takes
+// a share of the columns for all ranks, writes its sums into every other CTA's shared memory, and has its share of the outputs, whose first rows of `up` and of
+// base it loads before the barrier.  32 requests of as many adapters of rank 16 beside 4096 × 4096: 7.1 us a call (two launches, with the sums through the scratch:
+// 12.2; 8.4 MB at the rate of a copy: 1.3), one token beside 2048 × 2048: 5.5 (7.5), of which the call itself is the most.
+//
+// Prompts (tiles of 32): two launches, since base and output are most of the traffic and want CTAs of their own.  1501 rows of six requests, rank 64, beside 14336 × 4096:
+// 73 us, the first launch 22 of them, the second 52 for 195 MB; both are bound by the instructions around the copies and products, not by memory
+// (31 us) or by the tensor core (16).
 
 #include <cuda_fp16.h>
 
@@ -320,8 +323,8 @@ struct DownLayout {
     static constexpr uint32_t kRing = kStages * kStage, kBytes = (kRing > kMeet ? kRing : kMeet) + kSum;
 };
 
-// F16 adapters of ranks to 64: a row of v as fp16 terms, v · 2^e = hi + lo up to 2^-22 of v, with its largest number in [2^14, 2^15): products of fp16 numbers at
-// twice the rate of tf32 ones.  Numbers below 2^-16 of the row's largest would lose bits of lo: a row that has such (but not zero), or one that is not finite,
+// F16 adapters of ranks to 64 in the second launch: a row of v as fp16 terms, v · 2^e = hi + lo up to 2^-22 of v, with its largest number in [2^14, 2^15): products of fp16 numbers at
+// twice the rate of tf32 ones (62 -> 58 us for 1501 rows beside 14336).  Numbers below 2^-16 of the row's largest would lose bits of lo: a row that has such (but not zero), or one that is not finite,
 // stays as it is, with 0 as its scale.  `v`: this lane's four numbers of the row that kLanes lanes have; comes back as four hi and four lo, the inverse of 2^e in `scale`.
 template <uint32_t LANES>
 __device__ __forceinline__ float4 halves_of_row(const float4 &v, float *scale) {
@@ -499,6 +502,8 @@ __global__ void __launch_bounds__(kUpThreads, kUpCtas<T>) adapter_up_kernel(cons
         uint32_t n, adapter, out0, fresh;  // fresh: other rows of `up` than the block before
         uint32_t row[16];
         float row_scale[16];
+        uint32_t rank;
+        float scale;
     };
     extern __shared__ __align__(16) float4 copies[];  // [place][warp][base of four rows][lane], then [place][pieces of v: of two rows per step][lane]
     __shared__ Block blocks[kPlaces];
@@ -539,6 +544,12 @@ __global__ void __launch_bounds__(kUpThreads, kUpCtas<T>) adapter_up_kernel(cons
                 if (sizeof(T) == 2 && adapter != ~0u) copy_async<4>((uint32_t)__cvta_generic_to_shared(block.row_scale + before), p.row_scales + row0 + lane, true);
             }
             if (lane == 0) block.n = n, block.adapter = adapter, block.out0 = fresh, block.fresh = adapter != adapter_before || fresh != out_before;
+            if (n && adapter != ~0u && (adapter != adapter_before || fresh != out_before)) {  // rows of `up` that the compute warps will load
+                if (lane == 0) copy_async<4>((uint32_t)__cvta_generic_to_shared(&block.rank), p.ranks + adapter, true), copy_async<4>((uint32_t)__cvta_generic_to_shared(&block.scale), p.scales + adapter, true);
+                const char *up = static_cast<const char *>(p.up) + ((size_t)adapter * p.n_rows + fresh) * p.max_rank * sizeof(T);
+                const uint32_t bytes = min(kUpWarps * 32, p.n_rows - fresh) * p.max_rank * (uint32_t)sizeof(T);
+                for (uint32_t i = lane * 128; i < bytes; i += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(up + i));
+            }
             adapter_before = adapter, out_before = fresh;
             rows &= ~__ballot_sync(0xffffffffu, taken);
             __syncwarp();
@@ -596,8 +607,8 @@ __global__ void __launch_bounds__(kUpThreads, kUpCtas<T>) adapter_up_kernel(cons
         if (n == 0) return;
         scale = of == ~0u ? -0.f : scale;  // (-0 · 0 + base: its bits)
         if (block.fresh && of != ~0u) {
-            const uint32_t rank = min(__ldg(p.ranks + of), p.max_rank);
-            scale = __ldg(p.scales + of);
+            const uint32_t rank = min(block.rank, p.max_rank);
+            scale = block.scale;
             const T *first = static_cast<const T *>(p.up) + (size_t)of * p.n_rows * p.max_rank;
 #pragma unroll
             for (uint32_t j = 0; j < kUpSteps; j++) load_up(p, first, o, j, rank, up[j]);
@@ -713,7 +724,9 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_up_wide_kernel(const __gr
 }
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
-bool is_step(const AdapterBatch &a) { return a.batch <= 64; }
+// 128 rows of 4 (48) adapters of rank 16 and 64 beside 4096 × 4096 take 10.0, 14.3 (14.6, 26.0) us as a step and 18.4, 20.3 (52.6, 61.1) as prompts, 256 rows 15.2,
+// 20.5 (21.3, 36.4) and 17.2, 18.8 (33.2, 38.5).
+bool is_step(const AdapterBatch &a) { return a.batch <= 128; }
 uint32_t rank_pitch(const AdapterBatch &a) { return is_step(a) ? (a.max_rank + 3) / 4 * 4 : (a.max_rank + 15) / 16 * 16; }
 
 cudaError_t launch_cluster(void (*kern)(AdapterParams), dim3 grid, uint32_t ctas, size_t smem, bool pdl, cudaStream_t s, const AdapterParams &p) {
@@ -736,7 +749,10 @@ cudaError_t launch_cluster(void (*kern)(AdapterParams), dim3 grid, uint32_t ctas
 template <typename T>
 cudaError_t launch_step(const AdapterBatch &a, AdapterParams p, cudaStream_t s, uint64_t *launches) {
     const uint32_t tiles = ceil_div(a.batch, kStepRows), slots = a.batch < kStepRows ? a.batch : kStepRows;
-    const uint32_t ctas = tiles * slots <= 16 ? 16 : 8;
+    // Sixteen CTAs for a few clusters: one row of rank 64 beside 4096 × 14336 takes 10.2 us with them and 15.7 with eight, beside 2048 × 2048 7.1 and 7.4.  Sixteen clusters (if
+    // every row has an adapter of its own) gain from it where adapters are large, 17.9 us against 20.6 (small ones lose, 12.3 against 9.4), more never.
+    const uint64_t bytes = (uint64_t)a.max_rank * (a.n_cols + a.n_rows) * sizeof(T);  // of an adapter
+    const uint32_t ctas = tiles * slots <= 8 || (tiles * slots <= 16 && bytes >= (1u << 20)) ? 16 : 8;
     p.cols_per_cta = ceil_div(a.n_cols, ctas * kWarps * 16) * kWarps * 16;
     p.outs_per_cta = ceil_div(a.n_rows, ctas * 32) * 32;
     const size_t smem = (size_t)kStepRows * (ctas * p.rank_pitch + 2 * v_pitch(a.max_rank)) * sizeof(float);
@@ -749,7 +765,11 @@ cudaError_t launch_step(const AdapterBatch &a, AdapterParams p, cudaStream_t s, 
 template <typename T>
 cudaError_t launch_prompts(const AdapterBatch &a, AdapterParams p, int sm_count, cudaStream_t s, uint64_t *launches) {
     using L = DownLayout<T>;
-    const uint32_t tiles = ceil_div(a.batch, kTileRows), slots = a.n_adapters < 4 ? a.n_adapters : 4;
+    // Slots: CTAs without one leave at once (33.4 us for 1500 rows of six requests with 4 as with 16), tiles of many adapters are sooner done (1024 rows, 64 of them of 48
+    // adapters: 185 us with 4, 162 with 16, 168 with 32).
+    const uint32_t tiles = ceil_div(a.batch, kTileRows), slots = a.n_adapters < 16 ? a.n_adapters : 16;
+    // As many CTAs per tile as are there at once (1500 rows of 4096 columns: 59.8 us with two, 43.0 with four, 40.0 with the five of this rule, 46.0 with eight; 96 rows of
+    // 14336 columns: 66, 44, and 27 with eight).
     uint32_t ctas = 8;
     while (ctas > 1 && ((ctas - 1) * L::kCols >= a.n_cols || (uint64_t)tiles * ctas > 7 * (uint64_t)sm_count / 4)) ctas--;
     p.cols_per_cta = ceil_div(a.n_cols, ctas * L::kCols) * L::kCols;

@@ -40,8 +40,8 @@ __device__ __forceinline__ float4 load4(const float *at, bool there) { return th
 
 // A warp per tile of 16 positions, the positions as rows of the tensor core's first operand and the query rows as the eight columns of its second, so that a CTA with few
 // query rows multiplies few zeros.  K and V of a tile come to the warp's own shared memory by tiled bulk copies: the next tile's K is asked for when this one's scores are there, its V
-// when its output is.  (Loaded into registers they take as much of L1 while they are on their way, and beside prefix_tc_kernel there is none: 114 us where this takes
-// LATER.)  They are split where they are used; which position and which dimensions a lane has is chosen so that its loads are 16 bytes and meet no others' banks.
+// when its output is.  (Loaded into registers they take as much of L1 while they are on their way, and beside prefix_tc_kernel there is none: 114 us for 64
+// sequences of 64 heads behind 8192 positions where copies took 104.)  They are split where they are used; which position and which dimensions a lane has is chosen so that its loads are 16 bytes and meet no others' banks.
 // HD: head_dim rounded up, or head_dim itself (EXACT); ROWS: query rows in eights.
 template <int HD, int ROWS, bool EXACT>
 __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PartMaps maps) {
@@ -409,13 +409,15 @@ struct Cut {
 Cut shape_of(const PrefixAttention &a, int sm_count, PrefixParams *p) {
     const uint32_t group = a.n_heads / a.n_kv_heads, mine = a.n_query * group, all = a.n_seqs * mine;
     Cut cut;
-    cut.tc = prefix_tc_supported(a.hd) && all >= 32 && a.prefix_len >= 64;
-    if (const char *e = knob("YULE_PREFIX_TC")) cut.tc = prefix_tc_supported(a.hd) && atoi(e) != 0 && a.prefix_len > 0;
+    // The tensor core's accumulators take 128 rows whatever there is of them, and the copies of K and V in its form a launch: 4 to 5 us that have to be won back.
+    // Without it and with it, 32 heads of 128 (8 KV heads): 32 rows of 1024 positions 18.0 and 19.2 us, of 4096 33.5 and 28.2; 128 rows of 256 17.8 and 17.4, of 4096
+    // 85 and 33; 16 rows of 4096 24.6 and 27.9.  32 heads of 64 (4 KV heads): 128 rows of 1024 13.1 and 12.7, 256 rows of 4096 43 and 18.
+    cut.tc = prefix_tc_supported(a.hd) && all >= 32 && (uint64_t)all * a.prefix_len * a.n_kv_heads * a.hd >= (1u << 25);
     cut.rows = a.hd > 128 || mine <= 8 ? 1 : mine <= 16 ? 2 : 3;
     p->group = group;
-    // Chunks such that the CTAs are a few per SM, of at least one tile for every warp.
-    uint32_t want = 8 * sm_count;
-    if (const char *e = knob("YULE_PREFIX_WANT")) want = atoi(e) * sm_count;
+    // Chunks such that there are eight CTAs per SM, of at least one tile for every warp: 32 own caches of to 1000 positions behind a prefix of 64 take 72.8 us with one per SM,
+    // 49.6 with two, 40.4 with four, 36.5 with eight, 35.3 with sixteen, one of 4000 22.0, 18.8, 16.1, 19.7 and 19.8.
+    const uint32_t want = 8 * sm_count;
     auto chunk = [&](uint64_t units, uint32_t len) {
         const uint64_t per = units ? (want + units - 1) / units : 1;
         const uint64_t c = ((len + per - 1) / per + kTileKeys - 1) / kTileKeys * kTileKeys;
