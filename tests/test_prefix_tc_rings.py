@@ -36,27 +36,27 @@ def simulate(seed, n, k_wait=True, v_wait=True, alpha_wait=True, s_wait=True, o_
     alpha = [[None] * SUM for _ in range(2)]
     k_used, v_used, p_used, s_read, o_read, alpha_read = {-1, -2, -3}, {-1, -2}, {-1, -2}, [[-2 + b] * SOFT for b in range(2)], [[-1] * SUM for _ in range(PARTS)], [[-2 + b] * SUM for b in range(2)]
     rows, rows_read = [[[None] * 2 for _ in range(2)] for _ in range(4)], [[-1] * 2 for _ in range(4)]
-    queue, outputs, copies = [], [], []
+    queue, outputs, copies, value_copies = [], [], [], []
 
-    def loader():
-        def copy(to, used, j):
-            def go():
-                assert j - len(to) in used, "an operand overwritten before it was used"
-                to[j % len(to)] = j
-            return go
+    def copy(to, used, j):
+        def go():
+            assert j - len(to) in used, "an operand overwritten before it was used"
+            to[j % len(to)] = j
+        return go
 
-        for j in range(min(2, n)):
-            copies.extend([copy(K, k_used, j), k_full[j].arrive])
+    def keys():
+        for j in range(n):
+            if j >= 2 and k_wait:
+                yield lambda: k_empty[j % 3].over(j // 3 & 1 ^ 1)
+            copies.extend([copy(K, k_used, j), k_full[j % 3].arrive])
+            yield lambda: True
+
+    def values():
         for j in range(n):
             b, ph = j & 1, j >> 1 & 1
             if v_wait:
                 yield lambda: v_empty[b].over(ph ^ 1)
-            copies.extend([copy(V, v_used, j), v_full[b].arrive])
-            i = j + 2
-            if i < n:
-                if k_wait:
-                    yield lambda: k_empty[i % 3].over(i // 3 & 1 ^ 1)
-                copies.extend([copy(K, k_used, i), k_full[i % 3].arrive])
+            value_copies.extend([copy(V, v_used, j), v_full[b].arrive])
             yield lambda: True
 
     def softmax(w):
@@ -138,9 +138,9 @@ def simulate(seed, n, k_wait=True, v_wait=True, alpha_wait=True, s_wait=True, o_
                 o_read[part][w] = j
                 o_empty[part].arrive()
         yield lambda: l_full.over(0)
-        assert k_used >= set(range(n)) and v_used >= set(range(n)) and not queue and not outputs and not copies, "the operands' memory taken while they are in use"
+        assert k_used >= set(range(n)) and v_used >= set(range(n)) and not queue and not outputs and not copies and not value_copies, "the operands' memory taken while they are in use"
 
-    interleave(rng, [issue_scores(), issue_output(), loader()] + [softmax(w) for w in range(SOFT)] + [sums(w) for w in range(SUM)], [queue, outputs, copies])
+    interleave(rng, [issue_scores(), issue_output(), keys(), values()] + [softmax(w) for w in range(SOFT)] + [sums(w) for w in range(SUM)], [queue, outputs, copies, value_copies])
 
 
 @pytest.mark.parametrize("n", [1, 2, 3, 4, 9, 14])

@@ -55,11 +55,11 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
     uint32_t *q_hi = reinterpret_cast<uint32_t *>(sm), *q_lo = q_hi + kRows * kPitch;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t turned = (g >> 1) | ((g & 1u) << 2);  // g with its lowest bit as its highest: two neighbours are four rows, or pieces, apart
-    yule_pdl_launch_dependents();
     // Behind the prefix on the tensor core nothing here depends on it, and what came before it is over (it waited, and let this kernel start): only one CTA's end waits, so that who
     // waits for this kernel has waited for that one.
     const bool waits = !p.beside || (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1);
     if (!p.beside) yule_pdl_wait();
+    yule_pdl_launch_dependents();  // (behind the wait: prefix_operands_kernel counts on it)
 
     // which positions, for which rows: x the rows (of the prefix's first), y the KV head, z the chunk
     const uint32_t kvh = blockIdx.y, split = blockIdx.z;
@@ -473,18 +473,13 @@ cudaError_t launch_prefix_attention(const PrefixAttention &a, int sm_count, cuda
     p.part_ml = reinterpret_cast<float2 *>(p.part_o + parts * a.hd);
     p.status = a.status;
     const uint64_t out_rows = (uint64_t)a.n_seqs * a.n_query * a.n_heads;
-    p.beside = cut.tc;
     p.prefix_items = cut.tc ? 0 : p.prefix_splits ? p.prefix_row_tiles : 0;
     const uint64_t items = p.prefix_items + (p.tail_splits ? (uint64_t)a.n_seqs * p.tail_row_tiles : 0);
     const uint32_t splits = !cut.tc && p.prefix_splits > p.tail_splits ? p.prefix_splits : p.tail_splits;
     if (items > 0x7FFFFFFFu || out_rows > 0x7FFFFFFFu || a.n_kv_heads > 65535 || splits > 65535) return cudaErrorInvalidValue;
     cudaError_t e = cudaSuccess;
     bool pdl = a.pdl;
-    if (cut.tc) {
-        if ((e = launch_prefix_tc(p, static_cast<unsigned char *>(a.scratch) + parts_bytes(a, p), pdl, s, launches)) != cudaSuccess) return e;
-        pdl = true;
-    }
-    if (items) {
+    auto own = [&]() -> cudaError_t {
         alignas(64) PartMaps maps = {};
         auto map = [&](const float *at, uint64_t rows, size_t stride, CUtensorMap *to) {
             return cached_tensor_map_2d(at, 8, (uint64_t)a.n_kv_heads * a.hd / 2, rows, stride * 4, 16, kKeys, to, 128);
@@ -503,9 +498,21 @@ cudaError_t launch_prefix_attention(const PrefixAttention &a, int sm_count, cuda
         e = a.hd <= 64 ? launch_rows<64>(p, maps, cut.rows, n, pdl, s) : a.hd <= 96 ? launch_rows<96>(p, maps, cut.rows, n, pdl, s) : a.hd <= 128 ? launch_rows<128>(p, maps, cut.rows, n, pdl, s)
                                                                                                       : launch_part<256, 1, false>(p, maps, n, pdl, s);
         ++*launches;
-        if (e != cudaSuccess) return e;
+        pdl = true;
+        return e;
+    };
+    // What comes first?  A sequence's own positions fill the GPU at once and leave when their memory is read, and K and V are converted beside them; behind the prefix they run beside the
+    // tensor core, a CTA per SM.  First and last, us: 32 sequences of 32 heads of 128 behind 1024 positions, 30 of their own 23.0 and 25.7, 1000 46.2 and 51.5, behind
+    // 2048 26.3 and 27.8, 51.7 and 54.4, with 300 35.5 and 35.3; behind 8192 (67 MB) 52.6 and 49.3, with 1000 75.5 and 77.0; 64 of 64 heads behind 8192 82.3 and 74.3, 127.8 and 122.2;
+    // 64 of 32 heads of 64 behind 2048 (4 MB), 300 of their own, 23.6 and 26.9.
+    const bool own_first = items && cut.tc && (uint64_t)a.prefix_len * a.n_kv_heads * a.hd * 8 <= 24u << 20;
+    p.beside = cut.tc && !own_first, p.behind = own_first;
+    if (own_first && (e = own()) != cudaSuccess) return e;
+    if (cut.tc) {
+        if ((e = launch_prefix_tc(p, static_cast<unsigned char *>(a.scratch) + parts_bytes(a, p), pdl, s, launches)) != cudaSuccess) return e;
         pdl = true;
     }
+    if (items && !own_first && (e = own()) != cudaSuccess) return e;
     const dim3 grid(ceil_div(out_rows, 4));
     e = a.hd <= 128 ? launch_kernel(prefix_merge_kernel<1>, grid, dim3(128), 0, s, pdl, p) : launch_kernel(prefix_merge_kernel<2>, grid, dim3(128), 0, s, pdl, p);
     if (e == cudaSuccess) ++*launches;

@@ -16,7 +16,8 @@ struct PrefixParams {
     size_t q_stride, out_stride, prefix_stride, tail_stride;
     float scale;  // log2(e) / sqrt(hd)
     int *status;  // of bounded waits
-    bool beside;  // the launch before is prefix_tc_kernel
+    bool beside;  // prefix_part_kernel: the launch before is prefix_tc_kernel
+    bool behind;  // prefix_operands_kernel: the launch before is prefix_part_kernel
 };
 
 // The prefix for 128 query rows at a time on tcgen05 (prefix_attention_tc.cu): leaves the parts of slots [0, prefix_splits).  prefix_chunk is a multiple of 64, of at most 512 tiles of

@@ -10,7 +10,7 @@
 // finite: every row sees it.
 //
 // Roles (512 threads): eight warps do the soft-max (a thread per row and half a tile's positions), four add the output up (a thread per row), two issue the MMAs of scores and of
-// output (one that does both waits for either 2900 clocks a tile), one the bulk copies.  The query rows are in tensor memory; K has three buffers, V, scores and probabilities have two, and the scores of a tile are issued two tiles ahead of its output,
+// output (one that does both waits for either 2900 clocks a tile), two the bulk copies of K and of V.  The query rows are in tensor memory; K has three buffers, V, scores and probabilities have two, and the scores of a tile are issued two tiles ahead of its output,
 // which comes in parts of 64 dimensions: one is added up while the next is multiplied.  (Converting K and V where they are used took 5000 to 7400 clocks a tile and CTA, by
 // the soft-max warps or by eight more: the MMAs take 1536.)
 
@@ -30,7 +30,7 @@ namespace {
 constexpr int kRows = (int)kPrefixTcRows;  // query rows per CTA = TMEM lanes
 constexpr int kKeys = (int)kPrefixTcKeys;  // positions per tile
 constexpr int kThreads = 512;
-constexpr uint32_t kSumWarp = 8, kMmaWarp = 12, kLoadWarp = 13, kOutputWarp = 14;  // the first of each; soft-max from 0 on
+constexpr uint32_t kSumWarp = 8, kMmaWarp = 12, kKeyWarp = 13, kOutputWarp = 14, kValueWarp = 15;  // the first of each; soft-max from 0 on
 constexpr int kLaunchRegs = 96;  // registers per thread that 512 threads are launched with (the build checks that the kernels get them)
 constexpr int kSoftRegs = 96, kSumRegs = 168, kIssueRegs = 24;
 static_assert(2 * kSoftRegs + kSumRegs + kIssueRegs <= 4 * kLaunchRegs, "register split");
@@ -88,7 +88,9 @@ __global__ void __launch_bounds__(256) prefix_operands_kernel(const __grid_const
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y, at = (tile0 + blockIdx.x) * kKeys, keys = p.prefix_len - at;
     const size_t slot = (size_t)kvh * gridDim.x + blockIdx.x;
     const float *kc = p.prefix_k + (size_t)at * p.prefix_stride + (size_t)kvh * HD, *vc = p.prefix_v + (size_t)at * p.prefix_stride + (size_t)kvh * HD;
-    yule_pdl_wait();
+    // (behind the sequences' own positions, which it runs beside: they let it start when what came before them was over, and only one CTA's end waits for theirs)
+    const bool waits = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
+    if (!p.behind) yule_pdl_wait();
     yule_pdl_launch_dependents();
     // K: eight dimensions of a position; eight neighbouring lanes take eight positions (whole rows of core matrices), the four groups of a warp four steps of eight dimensions.
     // V: eight positions of a dimension; neighbouring lanes take neighbouring dimensions.
@@ -141,6 +143,7 @@ __global__ void __launch_bounds__(256) prefix_operands_kernel(const __grid_const
         *reinterpret_cast<uint4 *>(vd) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4 *>(vd + L::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
+    if (p.behind && waits) yule_pdl_wait();
 }
 
 template <int HD>
@@ -231,8 +234,8 @@ __global__ void __launch_bounds__(640, 1) prefix_tc_kernel(  // (so many threads
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    if (warp == kLoadWarp) yule_pdl_wait();
-    if (warp == kLoadWarp && lane == 0)  // (beside the query rows)
+    if (warp == kKeyWarp || warp == kValueWarp) yule_pdl_wait();
+    if (warp == kKeyWarp && lane == 0)  // (beside the query rows)
         for (uint32_t j = 0; j < 2 && j < n_tiles; j++) load(j, L::kOffK + j * 2 * L::kPlane, k_full + 8 * j, 0);
     if (warp < 4) {
         const uint4 *from = reinterpret_cast<const uint4 *>(q_words + r * L::kPitch);
@@ -311,18 +314,18 @@ __global__ void __launch_bounds__(640, 1) prefix_tc_kernel(  // (so many threads
                     __syncwarp();
                 });
             }
-        } else if (warp == kLoadWarp && lane == 0) {
+        } else if (warp == kKeyWarp && lane == 0) {
             RingPos kr;
             kr.advance(3), kr.advance(3);
-            for (uint32_t j = 0; j < n_tiles && ok; j++) {  // V of this tile, K of the one after the next
+            for (uint32_t j = 2; j < n_tiles && ok; j++, kr.advance(3)) {
+                ok = mbar_wait(k_empty + 8 * kr.s, kr.ph ^ 1u, abort_flag, p.status);
+                if (ok) load(j, L::kOffK + kr.s * 2 * L::kPlane, k_full + 8 * kr.s, 0);
+            }
+        } else if (warp == kValueWarp && lane == 0) {
+            for (uint32_t j = 0; j < n_tiles && ok; j++) {
                 const uint32_t b = j & 1u;
                 ok = mbar_wait(v_empty + 8 * b, ((j >> 1) & 1u) ^ 1u, abort_flag, p.status);
                 if (ok) load(j, L::kOffV + b * 2 * L::kPlane, v_full + 8 * b, 2 * L::kPlane);
-                if (j + 2 < n_tiles && ok) {
-                    ok = mbar_wait(k_empty + 8 * kr.s, kr.ph ^ 1u, abort_flag, p.status);
-                    if (ok) load(j + 2, L::kOffK + kr.s * 2 * L::kPlane, k_full + 8 * kr.s, 0);
-                    kr.advance(3);
-                }
             }
         }
     } else if (warp < kSumWarp) {
@@ -488,7 +491,7 @@ uint32_t chunks_at_a_time(const PrefixParams &p) {
 }
 
 template <int HD>
-cudaError_t launch_variant(const PrefixParams &p, void *scratch, bool pdl, cudaStream_t s, uint64_t *launches) {
+cudaError_t launch_variant(PrefixParams p, void *scratch, bool pdl, cudaStream_t s, uint64_t *launches) {
     auto kern = prefix_tc_kernel<HD>;
     static bool attr_done[64] = {};  // the opt-in for large dynamic shared memory belongs to the device
     static std::mutex mu;
@@ -518,6 +521,7 @@ cudaError_t launch_variant(const PrefixParams &p, void *scratch, bool pdl, cudaS
                               static_cast<const float2 *>(scales), slot0, n);
         if (e != cudaSuccess) return e;
         *launches += 2;
+        p.behind = false;
     }
     return cudaSuccess;
 }
