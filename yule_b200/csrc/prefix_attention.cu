@@ -80,6 +80,19 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
         slot += p.prefix_splits;
         line = b * p.tail_capacity;  // the sequence's first row
     }
+    // The query rows, all under way together and beside the length (one after the other: 8 sequences of five tokens took 30.9 us in all, 27.8 so).
+    constexpr int kEach = kRows * (HD / 4) / (kWarps * 32);
+    static_assert(kRows * (HD / 4) % (kWarps * 32) == 0, "pieces of the query rows");
+    float4 query[kEach];
+    {
+        uint32_t r = tid / (HD / 4), token = (row0 + r) / p.group, head = (row0 + r) % p.group;
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            const uint32_t e = tid + i * kWarps * 32, next = e / (HD / 4), d = e % (HD / 4) * 4;
+            for (head += next - r, r = next; head >= p.group; token++) head -= p.group;
+            query[i] = load4(p.q + (size_t)token * p.q_stride + (size_t)(kvh * p.group + head) * p.hd + d, row0 + r < n_rows && d < p.hd);
+        }
+    }
     if (key0 >= key1) {
         if (waits) yule_pdl_wait();
         return;
@@ -105,14 +118,14 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
         if (first < key1) copy(first, 0), copy(first, 1);
     }
     // query rows, in units of ln 2, as two terms
-    for (uint32_t i = tid; i < kRows * (HD / 4); i += kWarps * 32) {
-        const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4, row = row0 + r;
-        const float4 v = load4(p.q + (size_t)(row / p.group) * p.q_stride + (size_t)(kvh * p.group + row % p.group) * p.hd + d, row < n_rows && d < p.hd);
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const uint32_t e = tid + i * kWarps * 32, r = e / (HD / 4), d = e % (HD / 4) * 4;
         uint4 hi, lo;
-        split_tf32(v.x * p.scale, hi.x, lo.x);
-        split_tf32(v.y * p.scale, hi.y, lo.y);
-        split_tf32(v.z * p.scale, hi.z, lo.z);
-        split_tf32(v.w * p.scale, hi.w, lo.w);
+        split_tf32(query[i].x * p.scale, hi.x, lo.x);
+        split_tf32(query[i].y * p.scale, hi.y, lo.y);
+        split_tf32(query[i].z * p.scale, hi.z, lo.z);
+        split_tf32(query[i].w * p.scale, hi.w, lo.w);
         *reinterpret_cast<uint4 *>(q_hi + r * kPitch + d) = hi;
         *reinterpret_cast<uint4 *>(q_lo + r * kPitch + d) = lo;
     }
@@ -283,9 +296,12 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
                 *reinterpret_cast<float4 *>(part + r * HD + 32 * i + 4 * turned) = make_float4(o[n][i][0][c], o[n][i][0][2 + c], o[n][i][1][c], o[n][i][1][2 + c]);
         }
     __syncthreads();
-    for (uint32_t i = tid; i < kRows * (HD / 4); i += kWarps * 32) {
-        const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4, row = row0 + r;
-        if (row >= n_rows || d >= p.hd) continue;
+    uint32_t r = tid / (HD / 4), token = (row0 + r) / p.group, head = (row0 + r) % p.group;
+#pragma unroll 2
+    for (uint32_t e = tid; e < kRows * (HD / 4); e += kWarps * 32) {
+        const uint32_t next = e / (HD / 4), d = e % (HD / 4) * 4;
+        for (head += next - r, r = next; head >= p.group; token++) head -= p.group;
+        if (row0 + r >= n_rows || d >= p.hd) continue;
         float mx = -INFINITY, sum = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -297,7 +313,7 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
             sum = fmaf(f, ml[2 * (w * kRows + r) + 1], sum);
             acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y), acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
         }
-        const size_t at = ((size_t)(row / p.group) * p.n_heads + kvh * p.group + row % p.group) * p.slots + slot;
+        const size_t at = ((size_t)token * p.n_heads + kvh * p.group + head) * p.slots + slot;
         if (d == 0) p.part_ml[at] = make_float2(mx, sum);
         *reinterpret_cast<float4 *>(p.part_o + at * p.hd + d) = acc;
     }
@@ -419,7 +435,8 @@ Cut shape_of(const PrefixAttention &a, int sm_count, PrefixParams *p) {
     // Without it and with it, 32 heads of 128 (8 KV heads): 32 rows of 1024 positions 18.0 and 19.2 us, of 4096 33.5 and 28.2; 128 rows of 256 17.8 and 17.4, of 4096
     // 85 and 33; 16 rows of 4096 24.6 and 27.9.  32 heads of 64 (4 KV heads): 128 rows of 1024 13.1 and 12.7, 256 rows of 4096 43 and 18.
     cut.tc = prefix_tc_supported(a.hd) && all >= 32 && (uint64_t)all * a.prefix_len * a.n_kv_heads * a.hd >= (1u << 25);
-    cut.rows = a.hd > 128 || mine <= 8 ? 1 : mine <= 16 ? 2 : 3;
+    // (24 rows take 1.43 times as long as 16: 172 and 120 us for 64 sequences of eight tokens of 32 heads)
+    cut.rows = a.hd > 128 || mine <= 8 ? 1 : mine <= 16 || 1.43 * ceil_div(mine, 24) > ceil_div(mine, 16) ? 2 : 3;
     p->group = group;
     // Chunks such that there are eight CTAs per SM, of at least one tile for every warp: 32 own caches of to 1000 positions behind a prefix of 64 take 72.8 us with one per SM,
     // 49.6 with two, 40.4 with four, 36.5 with eight, 35.3 with sixteen, one of 4000 22.0, 18.8, 16.1, 19.7 and 19.8.
