@@ -256,15 +256,19 @@ class CudaB200Backend:
         heads, kv = n_heads * head_dim, n_kv_heads * head_dim
         shape = _lib.PrefixAttention(head_dim, n_heads, n_kv_heads, prefix_len, n_seqs, n_query, tail_capacity, heads if q_stride is None else q_stride,
                                      heads if out_stride is None else out_stride, kv if prefix_stride is None else prefix_stride, kv if tail_stride is None else tail_stride)
-        k, v, tk, tv, lens = (h.id if h else 0 for h in (prefix_k, prefix_v, tail_k, tail_v, tail_lens))
-        _check(self._lib.yule_cuda_prefix_attention(self._ctx, q.id, k, v, tk, tv, lens, out.id, C.byref(shape)))
+        rc = self._lib.yule_cuda_prefix_attention(self._ctx, q.id, prefix_k.id if prefix_k else 0, prefix_v.id if prefix_v else 0, tail_k.id if tail_k else 0,
+                                                  tail_v.id if tail_v else 0, tail_lens.id if tail_lens else 0, out.id, C.byref(shape))
+        if rc:
+            _check(rc)
 
     def adapter_matmul_batched(self, down: BufferHandle, up: BufferHandle, ranks: BufferHandle, scales: BufferHandle, row_adapter: BufferHandle, input: BufferHandle,
                                base: BufferHandle, output: BufferHandle, n_rows: int, n_cols: int, dtype: DType, n_adapters: int, max_rank: int, batch: int,
                                x_stride: int | None = None, out_stride: int | None = None) -> None:
         """``output[i] = base[i] + scales[a] * up[a] @ (down[a] @ input[i])`` with ``a = row_adapter[i]``; ``base`` may be ``output``."""
         shape = _lib.Adapters(int(dtype), n_adapters, max_rank, n_rows, n_cols, batch, n_cols if x_stride is None else x_stride, n_rows if out_stride is None else out_stride)
-        _check(self._lib.yule_cuda_adapter_matmul_batched(self._ctx, down.id, up.id, ranks.id, scales.id, row_adapter.id, input.id, base.id, output.id, C.byref(shape)))
+        rc = self._lib.yule_cuda_adapter_matmul_batched(self._ctx, down.id, up.id, ranks.id, scales.id, row_adapter.id, input.id, base.id, output.id, C.byref(shape))
+        if rc:
+            _check(rc)
 
     def verify_drafts(self, target_logits: BufferHandle, draft_logits: BufferHandle | None, drafts: BufferHandle, draft_lens: BufferHandle | None,
                       random: BufferHandle | None, out_tokens: BufferHandle, out_accepted: BufferHandle, vocab_size: int, n_seqs: int, n_draft: int,
@@ -272,8 +276,10 @@ class CudaB200Backend:
         """Which drafts stand, and the token after them.  ``draft_logits`` None: drafts that were not drawn from a distribution; ``draft_lens`` None: ``n_draft`` each."""
         shape = _lib.Verification(vocab_size, n_seqs, n_draft, vocab_size if target_stride is None else target_stride, vocab_size if draft_stride is None else draft_stride,
                                   temperature, 1 if greedy else 0)
-        q, lens, r = (h.id if h else 0 for h in (draft_logits, draft_lens, random))
-        _check(self._lib.yule_cuda_verify_drafts(self._ctx, target_logits.id, q, drafts.id, lens, r, out_tokens.id, out_accepted.id, C.byref(shape)))
+        rc = self._lib.yule_cuda_verify_drafts(self._ctx, target_logits.id, draft_logits.id if draft_logits else 0, drafts.id, draft_lens.id if draft_lens else 0,
+                                               random.id if random else 0, out_tokens.id, out_accepted.id, C.byref(shape))
+        if rc:
+            _check(rc)
 
     def buffer_address(self, handle: BufferHandle) -> int:
         """Device address of a buffer, for libraries that can look at memory of the same GPU; ``synchronize`` before and after."""

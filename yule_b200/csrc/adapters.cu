@@ -731,8 +731,7 @@ uint32_t rank_pitch(const AdapterBatch &a) { return is_step(a) ? (a.max_rank + 3
 
 cudaError_t launch_cluster(void (*kern)(AdapterParams), dim3 grid, uint32_t ctas, size_t smem, bool pdl, cudaStream_t s, const AdapterParams &p) {
     cudaError_t e;
-    if (ctas > 8 && (e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
-    if (smem > 24 * 1024 && (e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+    if ((ctas > 8 || smem > 24 * 1024) && (e = kernel_opt_in(reinterpret_cast<const void *>(kern), smem, ctas > 8)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid, cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -783,13 +782,13 @@ cudaError_t launch_prompts(const AdapterBatch &a, AdapterParams p, int sm_count,
         const uint64_t items = (uint64_t)tiles * ceil_div(a.n_rows, kUpWarps * 32), at_once = kUpCtas<T> * (uint64_t)sm_count;
         const size_t smem = (size_t)kPlaces * (kUpWarps * 4 + p.rank_pitch / 8) * 512;
         auto up = adapter_up_kernel<T>;
-        if ((e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+        if ((e = kernel_opt_in(reinterpret_cast<const void *>(up), smem, false)) != cudaSuccess) return e;
         e = launch_kernel(up, dim3((uint32_t)(items < at_once ? items : at_once)), dim3(kUpThreads), smem, s, true, p);
     } else {
         p.outs_per_cta = 2 * kPassOuts;
         const size_t smem = (size_t)2 * kTileRows * v_pitch(a.max_rank) * 4;
         auto up = adapter_up_wide_kernel<T>;
-        if ((e = cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+        if ((e = kernel_opt_in(reinterpret_cast<const void *>(up), smem, false)) != cudaSuccess) return e;
         e = launch_kernel(up, dim3(tiles, slots, ceil_div(a.n_rows, p.outs_per_cta)), dim3(kThreads), smem, s, true, p);
     }
     if (e == cudaSuccess) ++*launches;

@@ -17,6 +17,34 @@ namespace yule {
 
 static thread_local char g_err[512] = "";
 
+cudaError_t kernel_opt_in(const void *kernel, size_t smem, bool large_clusters) {
+    struct Done {
+        const void *kernel;
+        int device;
+        size_t smem;
+        bool large_clusters;
+    };
+    static std::vector<Done> all;
+    static std::mutex mu;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    Done *done = nullptr;
+    for (Done &d : all)
+        if (d.kernel == kernel && d.device == device) done = &d;
+    if (!done) all.push_back({kernel, device, 0, false}), done = &all.back();
+    if (smem > done->smem) {
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+        done->smem = smem;
+    }
+    if (large_clusters && !done->large_clusters) {
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+        done->large_clusters = true;
+    }
+    return cudaSuccess;
+}
+
 const char *knob(const char *name) {
     static const bool debug = [] {
         const char *d = getenv("YULE_CUDA_DEBUG");

@@ -410,7 +410,7 @@ cudaError_t launch_part(const PrefixParams &p, const PartMaps &maps, dim3 items,
     constexpr size_t smem = (size_t)kWarps * 2 * kKeys * HD * 4 + (query > meeting ? query : meeting);
     auto kern = prefix_part_kernel<HD, ROWS, EXACT>;
     if (smem > 47 * 1024) {  // (beside a kilobyte of its own)
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  // (of the current device)
+        const cudaError_t e = kernel_opt_in(reinterpret_cast<const void *>(kern), smem, false);
         if (e != cudaSuccess) return e;
     }
     return launch_kernel(kern, items, dim3(kWarps * 32), smem, s, pdl, p, maps);

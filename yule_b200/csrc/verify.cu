@@ -443,7 +443,7 @@ template <int CTAS, bool GREEDY>
 cudaError_t launch_variant(const VerifyParams &p, uint32_t n_seqs, bool pdl, cudaStream_t s) {
     auto kern = verify_kernel<CTAS, GREEDY>;
     if (CTAS > 8) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        const cudaError_t e = kernel_opt_in(reinterpret_cast<const void *>(kern), 0, true);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
