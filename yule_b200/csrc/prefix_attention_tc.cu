@@ -79,69 +79,62 @@ struct Layout {
     static_assert(kSmem <= 227 * 1024 && kOffBars % 8 == 0, "shared memory");
 };
 
-// A tile of K and V as the tensor core reads it, and its inverse scales.  Bound by memory: 16 bytes of each pair of elements.
+// A tile of K (z = 0) or of V as the tensor core reads it, and its inverse scale.  Bound by memory: 16 bytes of each pair of elements (8192 positions of 8 heads of
+// 128, 134 MB, 22 us).  (A CTA for both K and V has half as many on their way: 2048 positions 10.4 us, 8.2 so.)
 template <int HD>
 __global__ void __launch_bounds__(256) prefix_operands_kernel(const __grid_constant__ PrefixParams p, unsigned char *tiles, float2 *scales, uint32_t tile0) {
     using L = Layout<HD>;
-    constexpr int N = HD / 32;  // pieces of eight elements of each per thread
-    __shared__ uint32_t most_of[2][8];
+    constexpr int N = HD / 32;  // pieces of eight elements per thread
+    __shared__ uint32_t most_of[8];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y, at = (tile0 + blockIdx.x) * kKeys, keys = p.prefix_len - at;
+    const bool of_k = blockIdx.z == 0;
     const size_t slot = (size_t)kvh * gridDim.x + blockIdx.x;
-    const float *kc = p.prefix_k + (size_t)at * p.prefix_stride + (size_t)kvh * HD, *vc = p.prefix_v + (size_t)at * p.prefix_stride + (size_t)kvh * HD;
+    const float *from = (of_k ? p.prefix_k : p.prefix_v) + (size_t)at * p.prefix_stride + (size_t)kvh * HD;
     // (behind the sequences' own positions, which it runs beside: they let it start when what came before them was over, and only one CTA's end waits for theirs)
-    const bool waits = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
+    const bool waits = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
     if (!p.behind) yule_pdl_wait();
     yule_pdl_launch_dependents();
     // K: eight dimensions of a position; eight neighbouring lanes take eight positions (whole rows of core matrices), the four groups of a warp four steps of eight dimensions.
     // V: eight positions of a dimension; neighbouring lanes take neighbouring dimensions.
     const uint32_t key = warp * 8 + (lane & 7u), dim = tid % HD, first = tid / HD * 8;
-    float4 k[N][2];
-    float v[N][8], k_most = 0.f, v_most = 0.f;
+    float x[N][8], most = 0.f;
+    if (of_k) {
 #pragma unroll
-    for (uint32_t i = 0; i < N; i++) {
-        const float4 *src = reinterpret_cast<const float4 *>(kc + (size_t)key * p.prefix_stride + 32 * i + 8 * (lane >> 3));
-        k[i][0] = k[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (key < keys) k[i][0] = __ldcg(src), k[i][1] = __ldcg(src + 1);
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < N; i++)
-#pragma unroll
-        for (uint32_t e = 0; e < 8; e++) {
-            const uint32_t j = first + i * (256 / HD) * 8 + e;
-            v[i][e] = j < keys ? __ldcg(vc + (size_t)j * p.prefix_stride + dim) : 0.f;
+        for (uint32_t i = 0; i < N; i++) {
+            const float4 *src = reinterpret_cast<const float4 *>(from + (size_t)key * p.prefix_stride + 32 * i + 8 * (lane >> 3));
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+            if (key < keys) a = __ldcg(src), b = __ldcg(src + 1);
+            x[i][0] = a.x, x[i][1] = a.y, x[i][2] = a.z, x[i][3] = a.w, x[i][4] = b.x, x[i][5] = b.y, x[i][6] = b.z, x[i][7] = b.w;
         }
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
+        for (uint32_t i = 0; i < N; i++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) k_most = fmaxf(fmaxf(k_most, fmaxf(fabsf(k[i][e].x), fabsf(k[i][e].y))), fmaxf(fabsf(k[i][e].z), fabsf(k[i][e].w)));
-#pragma unroll
-        for (int e = 0; e < 8; e++) v_most = fmaxf(v_most, fabsf(v[i][e]));
+            for (uint32_t e = 0; e < 8; e++) {
+                const uint32_t j = first + i * (256 / HD) * 8 + e;
+                x[i][e] = j < keys ? __ldcg(from + (size_t)j * p.prefix_stride + dim) : 0.f;
+            }
     }
-    const uint32_t k_all = __reduce_max_sync(0xffffffffu, __float_as_uint(k_most)), v_all = __reduce_max_sync(0xffffffffu, __float_as_uint(v_most));
-    if (lane == 0) most_of[0][warp] = k_all, most_of[1][warp] = v_all;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(x[i][e]));
+    const uint32_t all = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+    if (lane == 0) most_of[warp] = all;
     __syncthreads();
-    float k_scale, v_scale, k_inv, v_inv;
-    pow2_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, most_of[0][lane & 7u])), k_scale, k_inv);
-    pow2_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, most_of[1][lane & 7u])), v_scale, v_inv);
-    if (tid == 0) scales[slot] = make_float2(k_inv, v_inv);
-    unsigned char *to = tiles + slot * L::kTile;
+    float scale, inv;
+    pow2_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, most_of[lane & 7u])), scale, inv);
+    if (tid == 0) (of_k ? scales[slot].x : scales[slot].y) = inv;
+    unsigned char *to = tiles + slot * L::kTile + (of_k ? 0 : 2 * L::kPlane);
+    const uint64_t two = pair(scale, scale);
 #pragma unroll
     for (uint32_t i = 0; i < N; i++) {
         uint32_t hi[4], lo[4];
-        const uint64_t ks = pair(k_scale, k_scale), vs = pair(v_scale, v_scale);
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            split2(mul2(pair(k[i][e].x, k[i][e].y), ks), hi[2 * e], lo[2 * e]);
-            split2(mul2(pair(k[i][e].z, k[i][e].w), ks), hi[2 * e + 1], lo[2 * e + 1]);
-        }
-        unsigned char *kd = to + (4 * i + (lane >> 3)) * (kKeys * 16) + key * 16;
-        *reinterpret_cast<uint4 *>(kd) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4 *>(kd + L::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-#pragma unroll
-        for (int e = 0; e < 4; e++) split2(mul2(pair(v[i][2 * e], v[i][2 * e + 1]), vs), hi[e], lo[e]);
-        unsigned char *vd = to + 2 * L::kPlane + (i * 256 + tid) * 16;
-        *reinterpret_cast<uint4 *>(vd) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4 *>(vd + L::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        for (int e = 0; e < 4; e++) split2(mul2(pair(x[i][2 * e], x[i][2 * e + 1]), two), hi[e], lo[e]);
+        unsigned char *d = to + (of_k ? (4 * i + (lane >> 3)) * (kKeys * 16) + key * 16 : (i * 256 + tid) * 16);
+        *reinterpret_cast<uint4 *>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4 *>(d + L::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     if (p.behind && waits) yule_pdl_wait();
 }
@@ -515,7 +508,7 @@ cudaError_t launch_variant(PrefixParams p, void *scratch, bool pdl, cudaStream_t
         const uint32_t n = all - tile0 < chunks * per_chunk ? all - tile0 : chunks * per_chunk;
         unsigned char *tiles = static_cast<unsigned char *>(scratch);
         float2 *scales = reinterpret_cast<float2 *>(tiles + (size_t)n * p.n_kv_heads * Layout<HD>::kTile);
-        e = launch_kernel(prefix_operands_kernel<HD>, dim3(n, p.n_kv_heads), dim3(256), 0, s, pdl || slot0 > 0, p, tiles, scales, tile0);
+        e = launch_kernel(prefix_operands_kernel<HD>, dim3(n, p.n_kv_heads, 2), dim3(256), 0, s, pdl || slot0 > 0, p, tiles, scales, tile0);
         if (e == cudaSuccess)
             e = launch_kernel(kern, dim3(chunks, p.prefix_row_tiles, p.n_kv_heads), dim3(kThreads), Layout<HD>::kSmem, s, true, p, static_cast<const unsigned char *>(tiles),
                               static_cast<const float2 *>(scales), slot0, n);
