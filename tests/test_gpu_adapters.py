@@ -99,6 +99,19 @@ def test_batches(backend, dtype, batch):
     go(backend, dtype=dtype, batch=batch, adapters=2, seed=batch, in_place=True)
 
 
+@pytest.mark.parametrize("batch", [1100, 1700, 2500, 4800])
+def test_long_prompts(backend, batch):
+    """As many CTAs to a tile as are there at once: from eight down to one; rows of an adapter in runs, and mixed ones at the start."""
+    ids = np.arange(batch) * 7 // batch
+    ids[:50] = np.arange(50) % 8
+    go(backend, batch=batch, rows=260, cols=320, adapters=7, rank=20, ids=ids, seed=batch)
+
+
+@BOTH
+def test_large_adapters_of_few_requests(backend, dtype):
+    go(backend, dtype=dtype, batch=12, rows=4100, cols=4096, adapters=9, rank=64)
+
+
 @pytest.mark.parametrize("batch", [6, 164])
 def test_order_of_the_rows_does_not_matter(backend, batch):
     """Neighbours of one adapter, all of one, all different, none at all."""

@@ -12,6 +12,17 @@ from yule_b200 import CudaB200Backend, YuleGpuError
 pytestmark = pytest.mark.gpu
 
 
+# Which kernels: by the rules, the prefix as parts, on the tensor core behind or before the sequences' own positions.
+ROUTES = {"rules": {}, "parts": {"YULE_PREFIX_TC": "0"}, "own first": {"YULE_PREFIX_TC": "1", "YULE_PREFIX_OWN_FIRST": "1"}, "own last": {"YULE_PREFIX_TC": "1", "YULE_PREFIX_OWN_FIRST": "0"}}
+
+
+@pytest.fixture(autouse=True, params=ROUTES)
+def route(request, monkeypatch):
+    for name, value in ROUTES[request.param].items():
+        monkeypatch.setenv(name, value)
+    return request.param
+
+
 def reference(q, pk, pv, tk, tv, lens):
     """q [B][T][H][hd], pk, pv [P][kv][hd], tk, tv [B][C][kv][hd] → (out, tolerance) [B][T][H][hd], [B][T][H]."""
     q, pk, pv, tk, tv = (np.asarray(a, np.float64) for a in (q, pk, pv, tk, tv))
@@ -251,6 +262,13 @@ def test_offsets_beyond_32_bits(backend):
     assert (np.abs(backend.download(h[2], q.size).reshape(q.shape) - out).max(-1) <= tol).all()
     for x in [tk, tv] + small + h:
         backend.free(x)
+
+
+def test_a_prefix_whose_operands_come_in_pieces(backend, route):
+    """70000 positions of 16 heads of 64: 573 MB as the tensor core reads them, of which 512 are in memory at a time."""
+    if route in ("rules", "parts"):
+        pytest.skip("no operands")
+    go(backend, B=2, H=16, kv=16, hd=64, P=70000, C=10)
 
 
 def test_refusals(backend):

@@ -24,16 +24,17 @@ cudaError_t kernel_opt_in(const void *kernel, size_t smem, bool large_clusters) 
         size_t smem;
         bool large_clusters;
     };
-    static std::vector<Done> all;
+    static Done all[64];  // (kernels times devices; beyond it the calls are made every time)
+    static int n = 0;
     static std::mutex mu;
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
     std::lock_guard<std::mutex> lock(mu);
-    Done *done = nullptr;
-    for (Done &d : all)
-        if (d.kernel == kernel && d.device == device) done = &d;
-    if (!done) all.push_back({kernel, device, 0, false}), done = &all.back();
+    Done here = {kernel, device, 0, false}, *done = &here;
+    for (int i = 0; i < n; i++)
+        if (all[i].kernel == kernel && all[i].device == device) done = &all[i];
+    if (done == &here && n < 64) all[n] = here, done = &all[n++];
     if (smem > done->smem) {
         if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
         done->smem = smem;
@@ -133,6 +134,11 @@ static int32_t ensure_batch_scratch(yule_cuda_ctx *ctx, size_t bytes) {
         Allowed() { cudaThreadExchangeStreamCaptureMode(&mode); }
         ~Allowed() { cudaThreadExchangeStreamCaptureMode(&mode); }
     } allowed;
+    try {
+        ctx->retired_scratch.reserve(ctx->retired_scratch.size() + 1);
+    } catch (const std::exception &) {
+        return fail(YULE_ERR_OUT_OF_MEMORY, "no host memory for the list of scratch blocks");
+    }
     void *block = nullptr;
     size_t got = bytes < 2 * ctx->batch_scratch_bytes ? 2 * ctx->batch_scratch_bytes : bytes;
     cudaError_t e = cudaMalloc(&block, got);

@@ -435,6 +435,7 @@ Cut shape_of(const PrefixAttention &a, int sm_count, PrefixParams *p) {
     // Without it and with it, 32 heads of 128 (8 KV heads): 32 rows of 1024 positions 18.0 and 19.2 us, of 4096 33.5 and 28.2; 128 rows of 256 17.8 and 17.4, of 4096
     // 85 and 33; 16 rows of 4096 24.6 and 27.9.  32 heads of 64 (4 KV heads): 128 rows of 1024 13.1 and 12.7, 256 rows of 4096 43 and 18.
     cut.tc = prefix_tc_supported(a.hd) && all >= 32 && (uint64_t)all * a.prefix_len * a.n_kv_heads * a.hd >= (1u << 25);
+    if (const char *e = knob("YULE_PREFIX_TC")) cut.tc = prefix_tc_supported(a.hd) && a.prefix_len > 0 && atoi(e) != 0;
     // (24 rows take 1.43 times as long as 16: 172 and 120 us for 64 sequences of eight tokens of 32 heads)
     cut.rows = a.hd > 128 || mine <= 8 ? 1 : mine <= 16 || 1.43 * ceil_div(mine, 24) > ceil_div(mine, 16) ? 2 : 3;
     p->group = group;
@@ -529,7 +530,8 @@ cudaError_t launch_prefix_attention(const PrefixAttention &a, int sm_count, cuda
     // tensor core, a CTA per SM.  First and last, us: 32 sequences of 32 heads of 128 behind 1024 positions, 30 of their own 23.0 and 25.7, 1000 46.2 and 51.5, behind
     // 2048 26.3 and 27.8, 51.7 and 54.4, with 300 35.5 and 35.3; behind 8192 (67 MB) 52.6 and 49.3, with 1000 75.5 and 77.0; 64 of 64 heads behind 8192 82.3 and 74.3, 127.8 and 122.2;
     // 64 of 32 heads of 64 behind 2048 (4 MB), 300 of their own, 23.6 and 26.9.
-    const bool own_first = items && cut.tc && (uint64_t)a.prefix_len * a.n_kv_heads * a.hd * 8 <= 24u << 20;
+    bool own_first = items && cut.tc && (uint64_t)a.prefix_len * a.n_kv_heads * a.hd * 8 <= 24u << 20;
+    if (const char *x = knob("YULE_PREFIX_OWN_FIRST")) own_first = items && cut.tc && atoi(x) != 0;
     p.beside = cut.tc && !own_first, p.behind = own_first;
     if (own_first && (e = own()) != cudaSuccess) return e;
     if (cut.tc) {
