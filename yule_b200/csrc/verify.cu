@@ -65,7 +65,6 @@ struct VerifyParams {
     const float *random;
     uint32_t *tokens, *accepted;
     uint32_t vocab, n_draft, group;
-    bool whole;  // rows begin on 16-byte boundaries
     size_t target_stride, draft_stride;
     double per_bit;  // log2(e) / temperature
 };
@@ -237,28 +236,27 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
                     most = m, sum = s;
                 };
                 float v[kBatch];
-                uint32_t i = lo + first;
-                if (p.whole) {
-                    for (i = lo + 4 * first; i + (kBatch - 4) * step + 4 <= hi; i += kBatch * step) {
+                const uint32_t head = min((4u - (uint32_t)((uintptr_t)(row + lo) / 4 & 3u)) & 3u, hi - lo);  // ahead of the first 16-byte boundary
+                if (head && warp % per_row == 0) {
 #pragma unroll
-                        for (int j = 0; j < kBatch; j += 4) {
-                            const float4 x = __ldg(reinterpret_cast<const float4 *>(row + i + j * step));
-                            v[j] = x.x, v[j + 1] = x.y, v[j + 2] = x.z, v[j + 3] = x.w;
-                        }
-                        add(v, [&](int j) { return i + (j & 3) + (j & ~3) * step; });
-                    }
-                    if (i < hi) {  // what is left
-                        auto index = [&](int j) { return i + (j & 3) + (j & ~3) * step; };
+                    for (int j = 0; j < kBatch; j++) v[j] = -INFINITY;
+                    if (lane < head) v[0] = __ldg(row + lo + lane);
+                    add(v, [&](int j) { return j == 0 && lane < head ? lo + lane : hi; });
+                }
+                uint32_t i = lo + head + 4 * first;
+                for (; i + (kBatch - 4) * step + 4 <= hi; i += kBatch * step) {
 #pragma unroll
-                        for (int j = 0; j < kBatch; j++) v[j] = index(j) < hi ? __ldg(row + index(j)) : -INFINITY;
-                        add(v, index);
+                    for (int j = 0; j < kBatch; j += 4) {
+                        const float4 x = __ldg(reinterpret_cast<const float4 *>(row + i + j * step));
+                        v[j] = x.x, v[j + 1] = x.y, v[j + 2] = x.z, v[j + 3] = x.w;
                     }
-                } else {
-                    for (; i < hi; i += kBatch * step) {
+                    add(v, [&](int j) { return i + (j & 3) + (j & ~3) * step; });
+                }
+                if (i < hi) {  // what is left
+                    auto index = [&](int j) { return i + (j & 3) + (j & ~3) * step; };
 #pragma unroll
-                        for (int j = 0; j < kBatch; j++) v[j] = i + j * step < hi ? __ldg(row + i + j * step) : -INFINITY;
-                        add(v, [&](int j) { return i + j * step; });
-                    }
+                    for (int j = 0; j < kBatch; j++) v[j] = index(j) < hi ? __ldg(row + index(j)) : -INFINITY;
+                    add(v, index);
                 }
             }
             if (GREEDY) {
@@ -477,7 +475,6 @@ cudaError_t launch_verify_drafts(const VerifyDrafts &a, int sm_count, cudaStream
     // 128256: 69, 71, 76, 84).
     p.group = 1;
     while (p.group < most && p.group * 2 * slice <= 65536 && p.group <= a.n_draft) p.group *= 2;
-    p.whole = a.target_stride % 4 == 0 && (!a.draft || a.draft_stride % 4 == 0);
     cudaError_t e;
     if (few) e = a.greedy ? launch_variant<16, true>(p, a.n_seqs, a.pdl, s) : launch_variant<16, false>(p, a.n_seqs, a.pdl, s);
     else e = a.greedy ? launch_variant<8, true>(p, a.n_seqs, a.pdl, s) : launch_variant<8, false>(p, a.n_seqs, a.pdl, s);
