@@ -8,7 +8,7 @@
 //
 // Decode steps (tiles of 8): one launch, a cluster of CTAs per slot.  What there is to read is an adapter's 0.1 to 2 MB, so time goes by in latency: a CTA takes
 // a share of the columns for all ranks, writes its sums into every other CTA's shared memory, and has its share of the outputs, whose first rows of `up` and of
-// base it loads before the barrier.  32 requests of as many adapters of rank 16 beside 4096 × 4096: 7.1 us a call (two launches, with the sums through the scratch:
+// base it loads before the barrier.  32 requests of as many adapters of rank 16 beside 4096 × 4096: 7.4 us a call (two launches, with the sums through the scratch:
 // 12.2; 8.4 MB at the rate of a copy: 1.3), one token beside 2048 × 2048: 5.5 (7.5), of which the call itself is the most.
 //
 // Prompts (tiles of 32): two launches, since base and output are most of the traffic and want CTAs of their own.  1501 rows of six requests, rank 64, beside 14336 × 4096:
@@ -43,6 +43,12 @@ struct AdapterParams {
     bool whole_ranks, whole_outs;  // rows of `up`, and of out and base, are on the boundaries of vectors of four
 };
 
+// (Not by the read-only path: a launch before this one, which this one may have started beside, can have written any input.)
+template <typename T>
+__device__ __forceinline__ T read(const T *at) {
+    return *at;
+}
+
 // A tile's rows by adapter: a lane per row, each warp for itself.
 struct Tile {
     uint32_t id, same, firsts;  // this row's adapter (~0: none), the rows that share it, the first row of each adapter
@@ -51,7 +57,7 @@ template <uint32_t ROWS>
 __device__ __forceinline__ Tile read_tile(const AdapterParams &p, uint32_t row0) {
     const uint32_t lane = threadIdx.x & 31, row = row0 + lane;
     Tile t;
-    t.id = lane < ROWS && row < p.batch ? __ldg(p.row_adapter + row) : ~0u;
+    t.id = lane < ROWS && row < p.batch ? read(p.row_adapter + row) : ~0u;
     if (t.id >= p.n_adapters) t.id = ~0u;
     t.same = __match_any_sync(0xffffffffu, t.id);
     t.firsts = __ballot_sync(0xffffffffu, t.id != ~0u && (uint32_t)__ffs(t.same) == lane + 1);
@@ -107,8 +113,8 @@ template <>
 struct Four<float> {
     float4 v;
     __device__ __forceinline__ void load(const float *at, int n, bool whole) {
-        if (whole && n >= 4) v = __ldg(reinterpret_cast<const float4 *>(at));
-        else v = make_float4(n > 0 ? __ldg(at) : 0.f, n > 1 ? __ldg(at + 1) : 0.f, n > 2 ? __ldg(at + 2) : 0.f, n > 3 ? __ldg(at + 3) : 0.f);
+        if (whole && n >= 4) v = read(reinterpret_cast<const float4 *>(at));
+        else v = make_float4(n > 0 ? read(at) : 0.f, n > 1 ? read(at + 1) : 0.f, n > 2 ? read(at + 2) : 0.f, n > 3 ? read(at + 3) : 0.f);
     }
     __device__ __forceinline__ float4 get() const { return v; }
 };
@@ -116,10 +122,10 @@ template <>
 struct Four<__half> {
     uint2 v;
     __device__ __forceinline__ void load(const __half *at, int n, bool whole) {
-        if (whole && n >= 4) v = __ldg(reinterpret_cast<const uint2 *>(at));
+        if (whole && n >= 4) v = read(reinterpret_cast<const uint2 *>(at));
         else {
             const unsigned short *bits = reinterpret_cast<const unsigned short *>(at);
-            auto one = [&](int i) -> uint32_t { return n > i ? __ldg(bits + i) : 0u; };
+            auto one = [&](int i) -> uint32_t { return n > i ? read(bits + i) : 0u; };
             v = make_uint2(one(0) | one(1) << 16, one(2) | one(3) << 16);
         }
     }
@@ -190,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_step_kernel(const __grid_
     auto started = cluster.barrier_arrive();  // (waited for before anything is written to another CTA)
     yule_pdl_launch_dependents();
     yule_pdl_wait();
-    const uint32_t near_rank = lane < p.n_adapters ? __ldg(p.ranks + lane) : 0u;  // (beside the rows' adapters, not behind them)
+    const uint32_t near_rank = lane < p.n_adapters ? read(p.ranks + lane) : 0u;  // (beside the rows' adapters, not behind them)
     const Tile tile = read_tile<kStepRows>(p, row0);
     if (slot_at >= __popc(tile.firsts)) {  // (the same for all the cluster)
         if (slot_at == 0) copy_base<kStepRows>(p, tile, row0, out0, out1, none_lists[warp]);
@@ -199,8 +205,8 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_step_kernel(const __grid_
     }
     const uint8_t *rows = lists[warp];
     const Slot slot = read_slot(tile, slot_at, lists[warp]);
-    const uint32_t near = __shfl_sync(0xffffffffu, near_rank, slot.adapter & 31), rank = min(slot.adapter < 32 ? near : __ldg(p.ranks + slot.adapter), p.max_rank);
-    const float scale = __ldg(p.scales + slot.adapter);
+    const uint32_t near = __shfl_sync(0xffffffffu, near_rank, slot.adapter & 31), rank = min(slot.adapter < 32 ? near : read(p.ranks + slot.adapter), p.max_rank);
+    const float scale = read(p.scales + slot.adapter);
     const T *down = static_cast<const T *>(p.down) + (size_t)slot.adapter * p.max_rank * p.n_cols, *up = static_cast<const T *>(p.up) + (size_t)slot.adapter * p.n_rows * p.max_rank;
     const uint32_t share = p.cols_per_cta / kWarps, col0 = (cta * kWarps + warp) * share, col1 = min(col0 + share, p.n_cols);
     const float *x = p.x + (size_t)(row0 + rows[g < slot.n ? g : 0]) * p.x_stride;
@@ -215,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_step_kernel(const __grid_
             for (int j = 0; j < kSteps; j++) {
                 const uint32_t c = base + 16 * j + 4 * t;
                 const bool in = c < col1;
-                xv[j] = in && g < slot.n ? __ldg(reinterpret_cast<const float4 *>(x + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                xv[j] = in && g < slot.n ? read(reinterpret_cast<const float4 *>(x + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int r = 0; r < RANKS; r++) {
                     const uint32_t k = k0 + 16 * r + g;
@@ -387,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_down_kernel(const __grid_
     const uint8_t *rows = lists[warp];
     for (uint32_t s = blockIdx.y; s < n_slots; s += gridDim.y) {
         const Slot slot = read_slot(tile, s, lists[warp]);
-        const uint32_t rank = min(__ldg(p.ranks + slot.adapter), p.max_rank);
+        const uint32_t rank = min(read(p.ranks + slot.adapter), p.max_rank);
         const T *down = static_cast<const T *>(p.down) + (size_t)slot.adapter * p.max_rank * p.n_cols;
         constexpr uint32_t kPerRow = L::kCols * sizeof(T) / W, kCopies = L::kRanks * kPerRow / kThreads;  // copies of a row of `down`, and of a thread
         const uint32_t x_col = threadIdx.x % 16 * 4, x_row = threadIdx.x / 16, w_col = threadIdx.x % kPerRow * (W / sizeof(T)), w_row = threadIdx.x / kPerRow;
@@ -517,7 +523,7 @@ __global__ void __launch_bounds__(kUpThreads, kUpCtas<T>) adapter_up_kernel(cons
         const uint64_t items = (uint64_t)tiles * ((p.n_rows + kUpWarps * 32 - 1) / (kUpWarps * 32)), begin = blockIdx.x * items / gridDim.x;
         uint32_t left = (uint32_t)((blockIdx.x + 1) * items / gridDim.x - begin), tile = (uint32_t)(begin % tiles), out0 = (uint32_t)(begin / tiles) * kUpWarps * 32;
         uint32_t firsts = 0, rows = 0, adapter = 0, id = 0, row0 = 0, fresh = 0;
-        auto read_id = [&](uint32_t of) { return of * kTileRows + lane < p.batch ? __ldg(p.row_adapter + of * kTileRows + lane) : 0u; };  // (looked at a tile later: nothing waits for it here)
+        auto read_id = [&](uint32_t of) { return of * kTileRows + lane < p.batch ? read(p.row_adapter + of * kTileRows + lane) : 0u; };  // (looked at a tile later: nothing waits for it here)
         uint32_t id_next = left ? read_id(tile) : 0u, adapter_before = kNoRow, out_before = 0;
         // The next block, its copies under way (an empty group behind the last one).
         auto fetch = [&](uint32_t place) {
@@ -679,8 +685,8 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_up_wide_kernel(const __gr
     const uint8_t *rows = lists[warp];
     for (uint32_t s = blockIdx.y; s < n_slots; s += gridDim.y) {
         const Slot slot = read_slot(tile, s, lists[warp]);
-        const uint32_t rank = min(__ldg(p.ranks + slot.adapter), p.max_rank), steps = (rank + 15) / 16;
-        const float scale = __ldg(p.scales + slot.adapter);
+        const uint32_t rank = min(read(p.ranks + slot.adapter), p.max_rank), steps = (rank + 15) / 16;
+        const float scale = read(p.scales + slot.adapter);
         const T *up = static_cast<const T *>(p.up) + (size_t)slot.adapter * p.n_rows * p.max_rank;
         __syncthreads();  // (the slot before has read its sums)
         for (uint32_t i = threadIdx.x; i < kTileRows * steps * 16; i += kThreads) {

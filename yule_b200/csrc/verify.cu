@@ -69,6 +69,12 @@ struct VerifyParams {
     double per_bit;  // log2(e) / temperature
 };
 
+// (Not by the read-only path: a launch before this one, which this one may have started beside, can have written any input.)
+template <typename T>
+__device__ __forceinline__ T read(const T *at) {
+    return *at;
+}
+
 // A logit as it counts: NaN as −infinity, +infinity as the largest number.
 __device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
 __device__ __forceinline__ float power(float x) {  // of two, to 2^-22; subnormal ones are nothing
@@ -167,19 +173,19 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
     const float per_bit = (float)p.per_bit;
     yule_pdl_launch_dependents();
     yule_pdl_wait();
-    const uint32_t k = p.lens ? min(__ldg(p.lens + b), p.n_draft) : p.n_draft;
+    const uint32_t k = p.lens ? min(read(p.lens + b), p.n_draft) : p.n_draft;
     const float *target = p.target + (size_t)b * (p.n_draft + 1) * p.target_stride, *draft = !GREEDY && p.draft ? p.draft + (size_t)b * p.n_draft * p.draft_stride : nullptr;
     for (uint32_t t = tid; t < k; t += kThreads) {
-        if (!GREEDY) sh.random[t] = __ldg(p.random + (size_t)b * (p.n_draft + 1) + t);
-        const uint32_t x = __ldg(p.drafts + (size_t)b * p.n_draft + t);
+        if (!GREEDY) sh.random[t] = read(p.random + (size_t)b * (p.n_draft + 1) + t);
+        const uint32_t x = read(p.drafts + (size_t)b * p.n_draft + t);
         const bool in = x < p.vocab;
         sh.drafts[t] = x;
-        sh.target_at[t] = in ? clean(__ldg(target + (size_t)t * p.target_stride + x)) : -INFINITY;
-        sh.draft_at[t] = in && draft ? clean(__ldg(draft + (size_t)t * p.draft_stride + x)) : -INFINITY;
+        sh.target_at[t] = in ? clean(read(target + (size_t)t * p.target_stride + x)) : -INFINITY;
+        sh.draft_at[t] = in && draft ? clean(read(draft + (size_t)t * p.draft_stride + x)) : -INFINITY;
     }
     if (tid == 0) {
         sh.pick = kNothing;
-        if (!GREEDY) sh.last_random = __ldg(p.random + (size_t)b * (p.n_draft + 1) + p.n_draft);
+        if (!GREEDY) sh.last_random = read(p.random + (size_t)b * (p.n_draft + 1) + p.n_draft);
     }
     cluster.barrier_wait(std::move(started));
 
@@ -240,14 +246,14 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
                 if (head && warp % per_row == 0) {
 #pragma unroll
                     for (int j = 0; j < kBatch; j++) v[j] = -INFINITY;
-                    if (lane < head) v[0] = __ldg(row + lo + lane);
+                    if (lane < head) v[0] = read(row + lo + lane);
                     add(v, [&](int j) { return j == 0 && lane < head ? lo + lane : hi; });
                 }
                 uint32_t i = lo + head + 4 * first;
                 for (; i + (kBatch - 4) * step + 4 <= hi; i += kBatch * step) {
 #pragma unroll
                     for (int j = 0; j < kBatch; j += 4) {
-                        const float4 x = __ldg(reinterpret_cast<const float4 *>(row + i + j * step));
+                        const float4 x = read(reinterpret_cast<const float4 *>(row + i + j * step));
                         v[j] = x.x, v[j + 1] = x.y, v[j + 2] = x.z, v[j + 3] = x.w;
                     }
                     add(v, [&](int j) { return i + (j & 3) + (j & ~3) * step; });
@@ -255,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
                 if (i < hi) {  // what is left
                     auto index = [&](int j) { return i + (j & 3) + (j & ~3) * step; };
 #pragma unroll
-                    for (int j = 0; j < kBatch; j++) v[j] = index(j) < hi ? __ldg(row + index(j)) : -INFINITY;
+                    for (int j = 0; j < kBatch; j++) v[j] = index(j) < hi ? read(row + index(j)) : -INFINITY;
                     add(v, index);
                 }
             }
@@ -330,8 +336,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
 #pragma unroll
                 for (int j = 0; j < kAhead; j++) {
                     const uint32_t i = i0 + j * 32;
-                    x[j] = i < i1 ? __ldg(pr + i) : -INFINITY;
-                    y[j] = qr && i < i1 ? __ldg(qr + i) : -INFINITY;
+                    x[j] = i < i1 ? read(pr + i) : -INFINITY;
+                    y[j] = qr && i < i1 ? read(qr + i) : -INFINITY;
                 }
             };
             load(lo + warp * share + lane);
@@ -400,8 +406,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
     // That share again, some consecutive tokens a thread: the first whose running sum passes the goal, else the last that is possible.
     const Weight wp(pm, p.per_bit), wq(qr ? qm : 0.f, p.per_bit);
     auto w_of = [&](uint32_t i) {
-        double w = wp(__ldg(pr + i));
-        if (qr) w = fma(-wq(__ldg(qr + i)), ratio, w);
+        double w = wp(read(pr + i));
+        if (qr) w = fma(-wq(read(qr + i)), ratio, w);
         return i == without || !(w > 0.0) ? 0.0 : w;
     };
     const uint32_t each = (share + kThreads - 1) / kThreads, s0 = min(lo + of_warp * share, hi), s1 = min(s0 + share, hi), i0 = min(s0 + tid * each, s1), i1 = min(i0 + each, s1);
