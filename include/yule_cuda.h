@@ -255,7 +255,8 @@ int32_t yule_cuda_embed_gather(yule_cuda_ctx *ctx, yule_buffer table, uint32_t g
  * tail_capacity counts as tail_capacity): query token t sees its own and earlier ones, tail_lens[b] - (n_query - 1 - t) positions, none if that is negative.
  * A row that sees nothing is zero.  Scores, soft-max and head grouping as yule_cuda_multihead_attention.  Handles of a prefix_len
  * or tail_capacity of 0 are not looked at.  A value that is not finite in a position that a row sees makes that row's output not finite; what a
- * row does not see does not count for it, whatever it holds.  head_dim a multiple of 4, at most 256; strides multiples of 4; n_query at most 64. */
+ * row does not see does not count for it, whatever it holds.  head_dim a multiple of 4, at most 256; strides multiples of 4; n_query at most 64, n_kv_heads
+ * at most 65535, prefix_len and n_seqs * tail_capacity at most 2^31 - 1. */
 typedef struct yule_prefix_attention {
     uint32_t head_dim, n_heads, n_kv_heads;
     uint32_t prefix_len, n_seqs, n_query, tail_capacity;
@@ -271,7 +272,7 @@ int32_t yule_cuda_prefix_attention(yule_cuda_ctx *ctx, yule_buffer q, yule_buffe
  * alone.  down: [n_adapters][max_rank][n_cols], up: [n_adapters][n_rows][max_rank], both F16 or F32 (gguf_type); ranks: n_adapters words, the
  * rank of each adapter (more than max_rank counts as max_rank; rows and columns beyond it are not used); scales: n_adapters floats; row_adapter: batch words; input
  * [batch][x_stride], base and output [batch][out_stride] floats.  Rows of one adapter need not be neighbours, but are cheaper so.  n_cols and x_stride
- * multiples of 4; max_rank at most 256. */
+ * multiples of 4; max_rank at most 256, n_rows at most 2^23. */
 typedef struct yule_adapters {
     uint32_t gguf_type, n_adapters, max_rank, n_rows, n_cols;
     uint32_t batch, x_stride, out_stride;
@@ -290,7 +291,8 @@ int32_t yule_cuda_adapter_matmul_batched(yule_cuda_ctx *ctx, yule_buffer down, y
  * index, sampler.rs:150-163), the token is that logit's; draft_logits, random and temperature are then not looked at.
  * out_tokens: [n_seqs][n_draft + 1] words, the accepted drafts, the token after them, then 0xFFFFFFFF; out_accepted: n_seqs words, the number of accepted
  * drafts.  A logit that is NaN or -infinity is a token that cannot be; a row of those accepts nothing and gives 0xFFFFFFFF; a draft outside the
- * vocabulary is not accepted.  Penalties and cut-offs of yule_cuda_sample are not applied. */
+ * vocabulary is not accepted.  Penalties and cut-offs of yule_cuda_sample are not applied.  vocab_size at most 2^24, n_seqs 65536, n_draft from 1 to 256,
+ * temperature from 1e-6 to 1e6. */
 typedef struct yule_verification {
     uint32_t vocab_size, n_seqs, n_draft;
     uint32_t target_stride, draft_stride;

@@ -3,6 +3,10 @@
 Tolerance.  A product of fp32 numbers is off by at most 2^-20 of its size on the tensor core, a sum of some tens of products in 24 bits by less than 2^-19 of the sum of
 their sizes, and there are two such sums one behind the other: 2^-17 of Σ_k |up| Σ_c |down| |x| · |scale|, and half a step of the output."""
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -232,6 +236,14 @@ def test_beside_a_quantised_projection(backend):
     assert (np.abs(got - out) <= tol).all()
     second = backend.download(y2, batch * rows).reshape(batch, rows)
     assert np.abs(second - got.astype(np.float64) @ W.T).max() <= 1e-5 * (np.abs(got) @ np.abs(W).T).max()
+
+
+def test_a_small_call_does_not_take_room_from_a_larger_one():
+    """The first calls of a process: sixteen CTAs with little shared memory, then eight with more."""
+    code = ("import sys; sys.path[:0] = [{!r}, {!r}]\nfrom test_gpu_adapters import CudaB200Backend, go\nb = CudaB200Backend(0)\n"
+            "for n, rank in ((1, 1), (91, 16), (1, 17), (91, 50), (8, 256), (100, 256)):\n    go(b, batch=n, rank=rank, adapters=12)\n")
+    here = os.path.dirname(os.path.abspath(__file__))
+    subprocess.run([sys.executable, "-c", code.format(here, os.path.dirname(here))], check=True, timeout=300)
 
 
 def test_refusals(backend):

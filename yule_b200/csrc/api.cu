@@ -35,7 +35,7 @@ cudaError_t kernel_opt_in(const void *kernel, size_t smem, bool large_clusters) 
     for (int i = 0; i < n; i++)
         if (all[i].kernel == kernel && all[i].device == device) done = &all[i];
     if (done == &here && n < 64) all[n] = here, done = &all[n++];
-    if (smem > done->smem) {
+    if (smem > 24 * 1024 && smem > done->smem) {  // (what is asked for is a limit too: asking for less than every kernel has would take it away)
         if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
         done->smem = smem;
     }

@@ -392,7 +392,7 @@ inline cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block
     return launch_config<KArgs...>(cfg, kernel, args...);
 }
 
-// What a kernel has to opt in to on the current device: dynamic shared memory beyond 48 KB, clusters of sixteen.  Asked for once (the call costs half a microsecond).
+// What a kernel has to opt in to on the current device: dynamic shared memory beyond 24 KB (48 with its own), clusters of sixteen.  Asked for once (the call costs half a microsecond).
 cudaError_t kernel_opt_in(const void *kernel, size_t smem, bool large_clusters);
 
 cudaError_t launch_dequantize(const uint8_t *w, uint32_t type, uint64_t n_blocks, float *out,
