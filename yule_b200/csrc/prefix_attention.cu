@@ -42,8 +42,8 @@ __device__ __forceinline__ float4 load4(const float *at, bool there) { return th
 // query rows multiplies few zeros.  K and V of a tile come to the warp's own shared memory by tiled bulk copies: the next tile's K is asked for when this one's scores are there, its V
 // when its output is.  (Loaded into registers they take as much of L1 while they are on their way, and beside prefix_tc_kernel there is none: 114 us for 64
 // sequences of 64 heads behind 8192 positions where copies took 104.)  They are split where they are used; which position and which dimensions a lane has is chosen so that its loads are 16 bytes and meet no others' banks.
-// HD: head_dim rounded up, or head_dim itself (EXACT); ROWS: query rows in eights.
-template <int HD, int ROWS, bool EXACT>
+// HD: head_dim rounded up, or head_dim itself (EXACT); ROWS: query rows in eights; SINGLE: all positions of a sequence (prefix, then its own), whose output the CTA leaves.
+template <int HD, int ROWS, bool EXACT, bool SINGLE>
 __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PartMaps maps) {
     extern __shared__ __align__(1024) unsigned char smem[];
     constexpr int kPitch = HD + 16;  // floats of a query row: lanes of two rows meet in different banks
@@ -93,29 +93,32 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
             query[i] = load4(p.q + (size_t)token * p.q_stride + (size_t)(kvh * p.group + head) * p.hd + d, row0 + r < n_rows && d < p.hd);
         }
     }
-    if (key0 >= key1) {
+    // The tiles: of the chunk, or of the prefix and behind them those of the sequence's own positions.
+    const uint32_t of_it = SINGLE ? (p.prefix_len + kKeys - 1) / kKeys : 0, n_tiles = of_it + (key1 > key0 ? (key1 - key0 + kKeys - 1) / kKeys : 0);
+    if (n_tiles == 0 && !SINGLE) {
         if (waits) yule_pdl_wait();
         return;
     }
     const uint32_t ring = smem_u32(smem) + warp * 2 * kHalf, bar = smem_u32(&bars[warp][0]);
     const unsigned char *mine = smem + warp * 2 * kHalf;
-    auto copy = [&](uint32_t base, uint32_t which) {  // by one lane: K (0) or V of the tile
-        const uint64_t map = reinterpret_cast<uint64_t>(&maps.m[(of_prefix ? 0 : 2) + which]);
+    auto copy = [&](uint32_t tile, uint32_t which) {  // by one lane: K (0) or V of the tile
+        const bool prefix = SINGLE ? tile < of_it : of_prefix;
+        const uint32_t at = SINGLE && prefix ? tile * kKeys : line + key0 + (tile - of_it) * kKeys;
+        const uint64_t map = reinterpret_cast<uint64_t>(&maps.m[(prefix ? 0 : 2) + which]);
         mbar_arrive_expect_tx(bar + 8 * which, kHalf);
 #pragma unroll
         for (uint32_t i = 0; i < HD / 32; i++)  // (elements of eight bytes)
             asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(ring + which * kHalf + i * (kKeys * 128)), "l"(map),
-                         "r"(bar + 8 * which), "r"(kvh * (p.hd / 2) + 16 * i), "r"(line + base)
+                         "r"(bar + 8 * which), "r"(kvh * (p.hd / 2) + 16 * i), "r"(at)
                          : "memory");
     };
-    const uint32_t first = key0 + warp * kKeys;
     if (lane == 0) {
         mbar_init(bar, 1);
         mbar_init(bar + 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
         if (tid == 0) gave_up = 0;
-        if (first < key1) copy(first, 0), copy(first, 1);
+        if (warp < n_tiles) copy(warp, 0), copy(warp, 1);
     }
     // query rows, in units of ln 2, as two terms
 #pragma unroll
@@ -149,9 +152,9 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
         return ok;
     };
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t base = first; base < key1; base += kTileKeys, phase ^= 1u) {
-        const bool whole = base + kKeys <= key1;  // (what lies behind, in the tile or the row, may be anything)
-        const bool in0 = base + turned < key1, in1 = base + turned + 8 < key1;
+    for (uint32_t tile = warp; tile < n_tiles; tile += kWarps, phase ^= 1u) {
+        const uint32_t n = SINGLE && tile < of_it ? p.prefix_len - tile * kKeys : key1 - key0 - (tile - of_it) * kKeys;  // positions from the tile's first on (what lies behind, in the tile or the row, may be anything)
+        const bool whole = n >= (uint32_t)kKeys, in0 = turned < n, in1 = turned + 8 < n;
         // Scores of positions base + turned and base + turned + 8.  The tensor core truncates what it adds to, so the large products of four steps at a time have sums of their own.
         // (With few query rows a sum of all small products would be a chain of as many steps as there are products: four sums.)
         constexpr int kSums = ROWS == 1 ? 4 : 1;
@@ -198,7 +201,7 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
                 for (int e = 0; e < 4; e++) s[n][e] += big[n][e];
         }
         __syncwarp();
-        if (lane == 0 && base + kTileKeys < key1) copy(base + kTileKeys, 0);
+        if (lane == 0 && tile + kWarps < n_tiles) copy(tile + kWarps, 0);
         // Soft-max of s[0], s[1] (the first position) and s[2], s[3] (the second) in rows 8n + 2t and 8n + 2t + 1.
         uint32_t ph[ROWS][4], pl[ROWS][4];
         float alpha[ROWS][2];
@@ -247,8 +250,8 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
                 float4 a = *reinterpret_cast<const float4 *>(at + ((turned ^ t) << 4)), b = *reinterpret_cast<const float4 *>(at + 4 * 128 + ((turned ^ (t + 4)) << 4));
                 if (!EXACT && 32 * i + 4 * turned >= p.hd) a = b = zero;
                 if (!whole) {
-                    if (base + 8 * u + t >= key1) a = zero;
-                    if (base + 8 * u + t + 4 >= key1) b = zero;
+                    if (8 * u + t >= n) a = zero;
+                    if (8 * u + t + 4 >= n) b = zero;
                 }
                 uint32_t ah[4], al[4], bh[4], bl[4];
                 split_tf32(a.x, ah[0], al[0]), split_tf32(a.y, ah[1], al[1]), split_tf32(a.z, ah[2], al[2]), split_tf32(a.w, ah[3], al[3]);
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
                     for (int e = 0; e < 4; e++) o[n][i][c][e] = fmaf(o[n][i][c][e], alpha[n][e & 1], fresh[n][c][e]);
         }
         __syncwarp();
-        if (lane == 0 && base + kTileKeys < key1) copy(base + kTileKeys, 1);
+        if (lane == 0 && tile + kWarps < n_tiles) copy(tile + kWarps, 1);
     }
     if (!ok) {  // gave up: the copies that are on their way have a moment to arrive (the status word says that nothing here counts)
         const long long t0 = clock64();
@@ -312,6 +315,11 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
             const float4 x = *reinterpret_cast<const float4 *>(part + (w * kRows + r) * HD + d);
             sum = fmaf(f, ml[2 * (w * kRows + r) + 1], sum);
             acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y), acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
+        }
+        if constexpr (SINGLE) {
+            const float inv = n_tiles ? 1.0f / sum : 0.f;
+            *reinterpret_cast<float4 *>(p.out + (size_t)token * p.out_stride + (size_t)(kvh * p.group + head) * p.hd + d) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            continue;
         }
         const size_t at = ((size_t)token * p.n_heads + kvh * p.group + head) * p.slots + slot;
         if (d == 0) p.part_ml[at] = make_float2(mx, sum);
@@ -404,21 +412,29 @@ __global__ void __launch_bounds__(128, 3) prefix_merge_kernel(const __grid_const
         if (4 * (lane + 32 * i) < p.hd) *reinterpret_cast<float4 *>(to + 4 * (lane + 32 * i)) = make_float4(o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv);
 }
 
-template <int HD, int ROWS, bool EXACT>
+template <int HD, int ROWS, bool EXACT, bool SINGLE = false>
 cudaError_t launch_part(const PrefixParams &p, const PartMaps &maps, dim3 items, bool pdl, cudaStream_t s) {
     constexpr size_t query = (size_t)2 * ROWS * 8 * (HD + 16) * 4, meeting = (size_t)kWarps * ROWS * 8 * (HD + 2) * 4;
     constexpr size_t smem = (size_t)kWarps * 2 * kKeys * HD * 4 + (query > meeting ? query : meeting);
-    auto kern = prefix_part_kernel<HD, ROWS, EXACT>;
+    auto kern = prefix_part_kernel<HD, ROWS, EXACT, SINGLE>;
     if (smem > 47 * 1024) {  // (beside a kilobyte of its own)
         const cudaError_t e = kernel_opt_in(reinterpret_cast<const void *>(kern), smem, false);
         if (e != cudaSuccess) return e;
     }
     return launch_kernel(kern, items, dim3(kWarps * 32), smem, s, pdl, p, maps);
 }
-template <int HD>
+template <int HD, bool EXACT>
 cudaError_t launch_rows(const PrefixParams &p, const PartMaps &maps, uint32_t rows, dim3 items, bool pdl, cudaStream_t s) {
-    if (p.hd == HD) return rows == 1 ? launch_part<HD, 1, true>(p, maps, items, pdl, s) : rows == 2 ? launch_part<HD, 2, true>(p, maps, items, pdl, s) : launch_part<HD, 3, true>(p, maps, items, pdl, s);
-    return rows == 1 ? launch_part<HD, 1, false>(p, maps, items, pdl, s) : rows == 2 ? launch_part<HD, 2, false>(p, maps, items, pdl, s) : launch_part<HD, 3, false>(p, maps, items, pdl, s);
+    if (p.single) return launch_part<HD, 1, EXACT, true>(p, maps, items, pdl, s);
+    if constexpr (HD <= 128) {
+        if (rows == 2) return launch_part<HD, 2, EXACT>(p, maps, items, pdl, s);
+        if (rows == 3) return launch_part<HD, 3, EXACT>(p, maps, items, pdl, s);
+    }
+    return launch_part<HD, 1, EXACT>(p, maps, items, pdl, s);
+}
+template <int HD>
+cudaError_t launch_dims(const PrefixParams &p, const PartMaps &maps, uint32_t rows, dim3 items, bool pdl, cudaStream_t s) {
+    return p.hd == HD ? launch_rows<HD, true>(p, maps, rows, items, pdl, s) : launch_rows<HD, false>(p, maps, rows, items, pdl, s);
 }
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
@@ -439,6 +455,17 @@ Cut shape_of(const PrefixAttention &a, int sm_count, PrefixParams *p) {
     // (24 rows take 1.43 times as long as 16: 172 and 120 us for 64 sequences of eight tokens of 32 heads)
     cut.rows = a.hd > 128 || mine <= 8 ? 1 : mine <= 16 || 1.43 * ceil_div(mine, 24) > ceil_div(mine, 16) ? 2 : 3;
     p->group = group;
+    // Few positions: all of a sequence in one CTA, and nothing to be added up.  A launch less, but 32 positions at a time: 4 sequences of 32 heads of 64, 92 positions 9.2 and 6.6 us,
+    // 124 9.2 and 8.3, 192 9.0 and 9.3; of 128, 32 positions 9.3 and 6.7, 92 9.4 and 8.2, 124 9.1 and 11.3.
+    const bool can = !cut.tc && a.n_query == 1 && mine <= 8;
+    p->single = can && ((uint64_t)a.prefix_len + a.tail_capacity) * a.hd <= 10240;
+    if (const char *e = knob("YULE_PREFIX_SINGLE")) p->single = can && atoi(e) != 0;
+    if (p->single) {
+        p->prefix_row_tiles = p->prefix_splits = p->slots = 0;
+        p->tail_row_tiles = p->tail_splits = 1;
+        p->tail_chunk = a.tail_capacity, p->prefix_chunk = a.prefix_len;
+        return cut;
+    }
     // Chunks such that there are eight CTAs per SM, of at least one tile for every warp: 32 own caches of to 1000 positions behind a prefix of 64 take 72.8 us with one per SM,
     // 49.6 with two, 40.4 with four, 36.5 with eight, 35.3 with sixteen, one of 4000 22.0, 18.8, 16.1, 19.7 and 19.8.
     const uint32_t want = 8 * sm_count;
@@ -509,19 +536,21 @@ cudaError_t launch_prefix_attention(const PrefixAttention &a, int sm_count, cuda
         auto map = [&](const float *at, uint64_t rows, size_t stride, CUtensorMap *to) {
             return cached_tensor_map_2d(at, 8, (uint64_t)a.n_kv_heads * a.hd / 2, rows, stride * 4, 16, kKeys, to, 128);
         };
-        if (p.prefix_items) {
+        if (p.prefix_items || (p.single && a.prefix_len)) {
             e = map(a.prefix_k, a.prefix_len, p.prefix_stride, &maps.m[0]);
             if (e == cudaSuccess) e = map(a.prefix_v, a.prefix_len, p.prefix_stride, &maps.m[1]);
         }
-        if (p.tail_splits && e == cudaSuccess) {
+        if (p.tail_splits && a.tail_capacity && e == cudaSuccess) {
             const uint64_t rows = (uint64_t)a.n_seqs * a.tail_capacity;
             e = map(a.tail_k, rows, p.tail_stride, &maps.m[2]);
             if (e == cudaSuccess) e = map(a.tail_v, rows, p.tail_stride, &maps.m[3]);
         }
         if (e != cudaSuccess) return e;
         const dim3 n((uint32_t)items, a.n_kv_heads, splits);
-        e = a.hd <= 64 ? launch_rows<64>(p, maps, cut.rows, n, pdl, s) : a.hd <= 96 ? launch_rows<96>(p, maps, cut.rows, n, pdl, s) : a.hd <= 128 ? launch_rows<128>(p, maps, cut.rows, n, pdl, s)
-                                                                                                      : launch_part<256, 1, false>(p, maps, n, pdl, s);
+        e = a.hd <= 64    ? launch_dims<64>(p, maps, cut.rows, n, pdl, s)
+            : a.hd <= 96  ? launch_dims<96>(p, maps, cut.rows, n, pdl, s)
+            : a.hd <= 128 ? launch_dims<128>(p, maps, cut.rows, n, pdl, s)
+                          : launch_rows<256, false>(p, maps, cut.rows, n, pdl, s);
         ++*launches;
         pdl = true;
         return e;
@@ -539,6 +568,7 @@ cudaError_t launch_prefix_attention(const PrefixAttention &a, int sm_count, cuda
         pdl = true;
     }
     if (items && !own_first && (e = own()) != cudaSuccess) return e;
+    if (p.single) return cudaSuccess;
     const dim3 grid(ceil_div(out_rows, 4));
     e = a.hd <= 128 ? launch_kernel(prefix_merge_kernel<1>, grid, dim3(128), 0, s, pdl, p) : launch_kernel(prefix_merge_kernel<2>, grid, dim3(128), 0, s, pdl, p);
     if (e == cudaSuccess) ++*launches;

@@ -17,6 +17,7 @@ struct PrefixParams {
     float scale;  // log2(e) / sqrt(hd)
     int *status;  // of bounded waits
     bool beside;  // prefix_part_kernel: the launch before is prefix_tc_kernel
+    bool single;  // prefix_part_kernel: a sequence's whole attention in one CTA, which leaves the output
     bool alone;   // prefix_merge_kernel: there is no launch before it
     bool behind;  // prefix_operands_kernel: the launch before is prefix_part_kernel
 };
