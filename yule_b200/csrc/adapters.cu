@@ -12,7 +12,7 @@
 // 12.2; 8.4 MB at the rate of a copy: 1.3), one token beside 2048 × 2048: 5.5 (7.5), of which the call itself is the most.
 //
 // Prompts (tiles of 32): two launches, since base and output are most of the traffic and want CTAs of their own.  1501 rows of six requests, rank 64, beside 14336 × 4096:
-// 73 us, the first launch 22 of them, the second 52 for 195 MB; both are bound by the instructions around the copies and products, not by memory
+// 71 us, the first launch 22 of them, the second 51 for 195 MB; both are bound by the instructions around the copies and products, not by memory
 // (31 us) or by the tensor core (16).
 
 #include <cuda_fp16.h>
@@ -496,8 +496,8 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_down_kernel(const __grid_
 
 // out of all rows, ranks to 64.  A CTA has 128 outputs of one tile after another (its part of all outputs of all tiles), a warp 32 of them, whose rows of `up` it keeps in
 // registers while the adapter stays the same.  Rows come in blocks of sixteen of an adapter.  A fifth warp finds them and has their base
-// and v copied into shared memory two blocks ahead; named barriers hand the places over and back.
-constexpr uint32_t kUpWarps = 4, kPlaces = 4, kAhead = 2, kUpSteps = 4, kNoRow = ~0u - 1, kUpThreads = (kUpWarps + 1) * 32;
+// and v copied into shared memory a block ahead (1501 rows beside 14336: 71.1 us in all, two ahead 72.4, three 81.6); named barriers hand the places over and back.
+constexpr uint32_t kUpWarps = 4, kPlaces = 4, kAhead = 1, kUpSteps = 4, kNoRow = ~0u - 1, kUpThreads = (kUpWarps + 1) * 32;
 __device__ __forceinline__ void barrier_sync(uint32_t id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kUpThreads) : "memory"); }
 __device__ __forceinline__ void barrier_arrive(uint32_t id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kUpThreads) : "memory"); }
 template <typename T>
