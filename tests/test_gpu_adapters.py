@@ -187,6 +187,19 @@ def test_sizes_within_a_rank(backend, dtype, batch):
     c.free(backend)
 
 
+@BOTH
+@pytest.mark.parametrize("batch", [9, 200])
+def test_errors_have_no_sign(backend, dtype, batch):
+    """Two products one behind the other.  A sum on the tensor core is cut off at most eight times, by 2^-24 of what it has by then in the mean, two thirds of the whole: 2^-21.6 in each product,
+    2^-20.6 in both, and what is rounded on either side adds up in squares.  Products that were all short by 2^-22 (F32: twice that) would leave as much in every output."""
+    c = Call(batch=batch, rows=512, cols=4096, rank=64, ranks=[64, 64, 64], dtype=dtype, ids=np.arange(batch) % 3)
+    c.base[:] = 0
+    c.upload(backend).run(backend)
+    out, _ = c.reference()
+    assert np.linalg.norm(c.got(backend) - out) <= 2.0 ** -20.5 * np.linalg.norm(out)
+    c.free(backend)
+
+
 def test_ranks_beyond_the_largest_count_as_it(backend):
     go(backend, ranks=[17, NONE, 16])
 

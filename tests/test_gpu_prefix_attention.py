@@ -152,6 +152,18 @@ def test_larger(backend):
     go(backend, B=40, T=3, H=16, kv=2, hd=128, P=1111, C=99, seed=2)
 
 
+@pytest.mark.parametrize("T,hd", [(1, 128), (1, 96), (3, 64), (8, 128)])
+def test_errors_have_no_sign(backend, T, hd):
+    """Over many positions.  Rounded terms are off by up to 2^-22 of a product on either side, a score of up to 16 in 32 bits by 2^-21: 2^-20 of the output's norm, where products that
+    are all short by 2^-22 would add 2^-22 times the score of 8 to 16 to every probability on one side."""
+    c = Call(B=2, T=T, H=8, kv=2, hd=hd, P=5000, C=300, lens=[300, 150], spread=1.3, seed=T)
+    c.pk += np.random.default_rng(9).standard_normal(c.pk.shape[1:]).astype(np.float32)
+    c.upload(backend).run(backend)
+    out, _ = reference(c.q, c.pk, c.pv, c.tk, c.tv, c.lens)
+    assert np.linalg.norm(c.got(backend) - out) <= 2.0 ** -20 * np.linalg.norm(out)
+    c.free(backend)
+
+
 def test_strides(backend):
     """Rows of all tensors further apart than they are long, with NaN between them."""
     go(backend, pad=12, B=3, T=2, P=100, C=40)
