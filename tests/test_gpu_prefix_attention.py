@@ -147,6 +147,32 @@ def test_a_prefix_that_is_not_finite(backend, where, value):
         assert not np.isfinite(got[:, :, :4, 5]).any()
 
 
+@pytest.mark.parametrize("where", ["tk", "tv"])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("T,hd", [(1, 64), (4, 64), (5, 96), (3, 160)])
+def test_own_positions_that_are_not_finite(backend, where, value, T, hd):
+    """One that all of a sequence's query tokens see, and each of the newest ones: the rows that see it are not finite (K: no number of them, whatever the sign of the query's
+    element), the others as they were."""
+    n = 40
+    c = Call(B=2, T=T, H=8, kv=2, hd=hd, P=30, C=50, lens=[n, 20])
+    c.q[:, :, ::2, 5], c.q[:, :, 1::2, 5] = 1.5, -1.5  # (of either sign against the position's element)
+    clean = reference(c.q, c.pk, c.pv, c.tk, c.tv, c.lens)
+    c.upload(backend)
+    for j in [3] + list(range(n - T, n)):
+        bad = getattr(c, where).copy()
+        bad[0, j, 0, 5] = value
+        backend.copy_to_device(bad, c.h[where])
+        c.run(backend)
+        got = c.got(backend)
+        sees = max(0, j - (n - T))  # the first query token that does
+        rows = got[0, sees:, :4]
+        assert not np.isfinite(rows if where == "tk" else rows[..., 5]).any()
+        rest = np.ones(got.shape[:3], bool)
+        rest[0, sees:, :4] = False
+        assert (np.abs(got - clean[0]).max(-1) <= clean[1])[rest].all()
+    c.free(backend)
+
+
 def test_larger(backend):
     go(backend, B=32, H=32, kv=8, hd=128, P=2048, C=200, seed=1)
     go(backend, B=40, T=3, H=16, kv=2, hd=128, P=1111, C=99, seed=2)

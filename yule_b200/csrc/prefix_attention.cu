@@ -357,12 +357,14 @@ __global__ void __launch_bounds__(128, 3) prefix_merge_kernel(const __grid_const
         for (int i = 0; i < N; i++) q[i] = load4(qp + 4 * (lane + 32 * i), 4 * (lane + 32 * i) < p.hd);
         for (uint32_t j = common; j < seen; j++) {
             const float *kr = p.tail_k + cache + j * p.tail_stride, *vr = p.tail_v + cache + j * p.tail_stride;
-            float s = 0.f;
+            float s = 0.f, finite = 0.f;  // (or NaN: an infinite score of either sign is one, as in the parts, where the terms of an infinity are)
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const float4 k = load4(kr + 4 * (lane + 32 * i), 4 * (lane + 32 * i) < p.hd);
                 s = fmaf(q[i].x, k.x, fmaf(q[i].y, k.y, fmaf(q[i].z, k.z, fmaf(q[i].w, k.w, s))));
+                finite = fmaf(0.f, k.x, fmaf(0.f, k.y, fmaf(0.f, k.z, fmaf(0.f, k.w, finite))));
             }
+            s += finite;
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
             s *= p.scale;
