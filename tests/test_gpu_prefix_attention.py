@@ -312,6 +312,35 @@ def test_a_prefix_whose_operands_come_in_pieces(backend, route):
     go(backend, B=2, H=16, kv=16, hd=64, P=70000, C=10)
 
 
+def test_more_rows_than_one_grid_of_the_tensor_core_takes(backend, route):
+    """8392704 query rows of a KV head, 2.1 GB: zeros (every output is the mean of V) but for some rows."""
+    if route not in ("rules", "own first"):
+        pytest.skip("the same kernels")
+    B, T, H, hd, P = 2049, 64, 64, 64, 3
+    rng = np.random.default_rng(6)
+    pk, pv = (rng.standard_normal((P, 1, hd)).astype(np.float32) for _ in range(2))
+    rows, floats = B * T * H, B * T * H * hd
+    q, out = backend.allocate(floats * 4), backend.allocate(floats * 4)
+    at = [0, 8388480 - 8, 8388480, rows - 8]  # eights of rows
+    x = rng.standard_normal((len(at), 8, hd)).astype(np.float32)
+    small = backend.upload(x)
+    for i, row in enumerate(at):
+        backend.copy_buffer_offset(small, q, i * 8 * hd * 4, row * hd * 4, 8 * hd * 4)
+    h = [backend.upload(pk), backend.upload(pv)]
+    backend.prefix_attention(q, h[0], h[1], None, None, None, out, hd, H, 1, P, B, 0, n_query=T)
+    want, tol = reference(x.reshape(len(at), 1, 8, hd), pk, pv, np.zeros((len(at), 0, 1, hd)), np.zeros((len(at), 0, 1, hd)), np.zeros(len(at)))
+    mean, around = reference(np.zeros((1, 1, 1, hd)), pk, pv, np.zeros((1, 0, 1, hd)), np.zeros((1, 0, 1, hd)), [0])
+    piece = 16 * hd
+    for i, row in enumerate(at):
+        backend.copy_buffer_offset(out, small, row * hd * 4, 0, 8 * hd * 4)
+        assert (np.abs(backend.download(small, 8 * hd).reshape(8, hd) - want[i, 0]).max(-1) <= tol[i, 0]).all()
+    for row in (8, 1 << 20, 8388480 - 24, 8388480 + 8, rows - 24):
+        backend.copy_buffer_offset(out, small, row * hd * 4, 0, piece * 4)
+        assert (np.abs(backend.download(small, piece).reshape(16, hd) - mean[0, 0]).max(-1) <= around[0, 0]).all()
+    for b in [q, out, small] + h:
+        backend.free(b)
+
+
 def test_refusals(backend):
     c = Call().upload(backend)
     good = [c.h["q"], c.h["pk"], c.h["pv"], c.h["tk"], c.h["tv"], c.h["lens"], c.h["out"], 64, 8, 2, 70, 3, 50]

@@ -452,8 +452,8 @@ Cut shape_of(const PrefixAttention &a, int sm_count, PrefixParams *p) {
     // The tensor core's accumulators take 128 rows whatever there is of them, and the copies of K and V in its form a launch: 4 to 5 us that have to be won back.
     // Without it and with it, 32 heads of 128 (8 KV heads): 32 rows of 1024 positions 18.0 and 19.2 us, of 4096 33.5 and 28.2; 128 rows of 256 17.8 and 17.4, of 4096
     // 85 and 33; 16 rows of 4096 24.6 and 27.9.  32 heads of 64 (4 KV heads): 128 rows of 1024 13.1 and 12.7, 256 rows of 4096 43 and 18.
-    cut.tc = prefix_tc_supported(a.hd) && all >= 32 && (uint64_t)all * a.prefix_len * a.n_kv_heads * a.hd >= (1u << 25);
-    if (const char *e = knob("YULE_PREFIX_TC")) cut.tc = prefix_tc_supported(a.hd) && a.prefix_len > 0 && atoi(e) != 0;
+    cut.tc = prefix_tc_supported(a.hd, all) && all >= 32 && (uint64_t)all * a.prefix_len * a.n_kv_heads * a.hd >= (1u << 25);
+    if (const char *e = knob("YULE_PREFIX_TC")) cut.tc = prefix_tc_supported(a.hd, all) && a.prefix_len > 0 && atoi(e) != 0;
     // (24 rows take 1.43 times as long as 16: 172 and 120 us for 64 sequences of eight tokens of 32 heads)
     cut.rows = a.hd > 128 || mine <= 8 ? 1 : mine <= 16 || 1.43 * ceil_div(mine, 24) > ceil_div(mine, 16) ? 2 : 3;
     p->group = group;

@@ -25,7 +25,7 @@ struct PrefixParams {
 // The prefix for 128 query rows at a time on tcgen05 (prefix_attention_tc.cu): leaves the parts of slots [0, prefix_splits).  prefix_chunk is a multiple of 64, of at most 512 tiles of
 // 64; head_dim 64 or 128; `scratch` on a 128-byte boundary.
 constexpr uint32_t kPrefixTcRows = 128, kPrefixTcKeys = 64, kPrefixTcTiles = 512;
-bool prefix_tc_supported(uint32_t hd);
+bool prefix_tc_supported(uint32_t hd, uint64_t rows);  // rows: query rows of a KV head, as many as a grid takes
 size_t prefix_tc_scratch_bytes(const PrefixParams &p);
 cudaError_t launch_prefix_tc(const PrefixParams &p, void *scratch, bool pdl, cudaStream_t s, uint64_t *launches);
 

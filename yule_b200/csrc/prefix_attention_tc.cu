@@ -521,7 +521,7 @@ cudaError_t launch_variant(PrefixParams p, void *scratch, bool pdl, cudaStream_t
 
 }  // namespace
 
-bool prefix_tc_supported(uint32_t hd) { return hd == 64 || hd == 128; }
+bool prefix_tc_supported(uint32_t hd, uint64_t rows) { return (hd == 64 || hd == 128) && rows <= 65535ull * kPrefixTcRows; }
 
 size_t prefix_tc_scratch_bytes(const PrefixParams &p) {
     const size_t tiles = (size_t)(p.prefix_len + kKeys - 1) / kKeys, most = (size_t)chunks_at_a_time(p) * (p.prefix_chunk / kKeys);
