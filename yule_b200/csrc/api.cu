@@ -12,38 +12,22 @@
 
 #include "batch_args.h"
 #include "internal.h"
+#include "opt_in.h"
 
 namespace yule {
 
 static thread_local char g_err[512] = "";
 
 cudaError_t kernel_opt_in(const void *kernel, size_t smem, bool large_clusters) {
-    struct Done {
-        const void *kernel;
-        int device;
-        size_t smem;
-        bool large_clusters;
-    };
-    static Done all[64];  // (kernels times devices; beyond it the calls are made every time)
-    static int n = 0;
-    static std::mutex mu;
+    static OptIns opt_ins;
     int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
+    const cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
-    std::lock_guard<std::mutex> lock(mu);
-    Done here = {kernel, device, 0, false}, *done = &here;
-    for (int i = 0; i < n; i++)
-        if (all[i].kernel == kernel && all[i].device == device) done = &all[i];
-    if (done == &here && n < 64) all[n] = here, done = &all[n++];
-    if (smem > 24 * 1024 && smem > done->smem) {  // (what is asked for is a limit too: asking for less than every kernel has would take it away)
-        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
-        done->smem = smem;
-    }
-    if (large_clusters && !done->large_clusters) {
-        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
-        done->large_clusters = true;
-    }
-    return cudaSuccess;
+    // (what is asked for is a limit too: asking for less than every kernel has would take it away)
+    return opt_ins.take(
+        kernel, device, smem > 24 * 1024 ? smem : 0, large_clusters,
+        [&](size_t bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes); },
+        [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); }, cudaErrorMemoryAllocation);
 }
 
 const char *knob(const char *name) {
