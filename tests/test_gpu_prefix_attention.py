@@ -341,6 +341,18 @@ def test_more_rows_than_one_grid_of_the_tensor_core_takes(backend, route):
         backend.free(b)
 
 
+def test_handles_that_are_not_looked_at(backend):
+    """Those of caches without positions may be anything, the output's among them."""
+    c = Call(B=2, P=0, C=30, lens=[30, 11]).upload(backend)
+    c.h["pk"] = c.h["pv"] = c.h["out"]
+    c.run(backend)
+    c.check(backend)
+    c = Call(B=2, P=40, C=0, lens=[0, 0]).upload(backend)
+    c.h["tk"] = c.h["tv"] = c.h["lens"] = c.h["out"]
+    c.run(backend)
+    c.check(backend)
+
+
 def test_refusals(backend):
     c = Call().upload(backend)
     good = [c.h["q"], c.h["pk"], c.h["pv"], c.h["tk"], c.h["tv"], c.h["lens"], c.h["out"], 64, 8, 2, 70, 3, 50]

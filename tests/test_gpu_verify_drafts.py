@@ -275,6 +275,14 @@ def test_captured_and_replayed_with_other_inputs(backend):
     backend.graph_destroy(g)
 
 
+def test_handles_that_are_not_looked_at(backend):
+    """Greedy: draft logits and random numbers may be anything, an output among them."""
+    c = Call(by="lookup", greedy=True).upload(backend)
+    c.h["draft"], c.h["random"] = c.h["tokens"], c.h["accepted"]
+    c.run(backend)
+    c.check(backend)
+
+
 def test_refusals(backend):
     c = Call(lens=[1, 2, 3, 3]).upload(backend)
     h = c.h

@@ -1042,7 +1042,7 @@ int32_t yule_cuda_prefix_attention(yule_cuda_ctx *ctx, yule_buffer q, yule_buffe
     CTX_ENQUEUE(ctx);
     PrefixNeeds need;
     if (int32_t rc = check_prefix_attention(shape, &need)) return rc;
-    if (out == q || out == prefix_k || out == prefix_v || out == tail_k || out == tail_v || out == tail_lens)
+    if (out == q || (shape->prefix_len && (out == prefix_k || out == prefix_v)) || (shape->tail_capacity && (out == tail_k || out == tail_v || out == tail_lens)))
         return fail(YULE_ERR_INVALID_ARGUMENT, "the output of prefix_attention cannot be one of its inputs");
     FIND(ctx, q, Q);
     FIND(ctx, out, O);
@@ -1121,7 +1121,7 @@ int32_t yule_cuda_verify_drafts(yule_cuda_ctx *ctx, yule_buffer target_logits, y
     CTX_ENQUEUE(ctx);
     VerifyNeeds need;
     if (int32_t rc = check_verification(shape, draft_logits != 0, &need)) return rc;
-    for (yule_buffer in : {target_logits, draft_logits, drafts, draft_lens, random})
+    for (yule_buffer in : {target_logits, shape->greedy ? 0 : draft_logits, drafts, draft_lens, shape->greedy ? 0 : random})
         if (in && (in == out_tokens || in == out_accepted)) return fail(YULE_ERR_INVALID_ARGUMENT, "an output of verify_drafts cannot be one of its inputs");
     if (out_tokens == out_accepted) return fail(YULE_ERR_INVALID_ARGUMENT, "verify_drafts has two outputs, in a buffer each");
     FIND(ctx, target_logits, T);
