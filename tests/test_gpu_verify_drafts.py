@@ -233,6 +233,25 @@ def test_random_numbers_at_the_ends(backend):
             assert accepted[b] <= 3 and tokens[b, accepted[b]] < 300 and (tokens[b, accepted[b] + 1:] == NONE).all()
 
 
+@pytest.mark.parametrize("bits", [100, 125, 130, 135, 137, 160, 700])
+def test_drafts_that_are_next_to_impossible(backend, bits):
+    """p of a draft is 2^-bits or some bits less, and its random number times q 0.1 % of that above or below it: where probabilities have few bits in fp32, or none."""
+    B, V = 256, 300
+    c = Call(B=B, K=1, V=V, temperature=1.0, spread=1.0, near=0.3)
+    r = np.random.default_rng(bits)
+    x = r.integers(0, V, B)
+    c.drafts[:, 0] = x
+    b = np.arange(B)
+    c.target[b, 0, x] = -bits * np.log(2) + r.random(B)
+    c.draft[b, 0, x] = c.target[b, 0, x] + 0.5
+    p, q = (np.array([soft(row, 1.0)[i] for row, i in zip(a[:, 0], x)]) for a in (c.target, c.draft))
+    above = r.random(B) < 0.5
+    c.random[:, 0] = np.where(above, 1.001, 0.999) * p / q
+    assert (c.random[:, 0] > 0).all() and (c.random[:, 0] < 1).all()
+    c.upload(backend).run(backend)
+    assert (c.check(backend) == ~above).all()
+
+
 def test_greedy_ties_go_to_the_highest_index(backend):
     c = Call(B=2, K=2, V=9000, by="lookup", greedy=True)
     c.target[:] = 0

@@ -12,7 +12,7 @@
 //
 // A pick next to a border has to be the same however the sums are formed: in 32 bits the running sum over 128256 tokens is off by 1e-7 where a token has 8e-6 on
 // average, one pick in a hundred.  So w and its sums are in 64 bits (exponentials to 2^-34, see Weight), for the two rows that the token is drawn from.  The
-// comparisons before it are in 32 bits, good to 2^-16, and made again in 64 where the two sides are nearer than 2^-13 of one another.
+// comparisons before it are in 32 bits, good to 2^-16, and made again in 64 where the two sides are nearer than 2^-13 of one another, or both below 2^-100.
 //
 // w takes one pass over its two rows, although it needs the sums of both first: with the ratio of the sums known to 2^-16, tokens with p > q are told from the others,
 // and Σ w over them is Σ exp_p − ratio · Σ exp_q with the ratio known by then.  A token on the wrong side has |p − q| below 2^-16 of p, so with the mass of all
@@ -37,6 +37,7 @@ constexpr uint32_t kNothing = 0xFFFFFFFFu;
 constexpr int kBatch = 16;           // logits of a row that a thread has on their way
 constexpr int kAhead = 4;            // and of the rows that it draws from
 constexpr float kNear = 0x1p-13f;
+constexpr float kFewBits = 0x1p-100f;  // less, and a product or quotient on the way can have been subnormal
 
 __device__ __forceinline__ uint64_t pair(float a, float b) {
     uint64_t r;
@@ -311,8 +312,9 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
                 const float px = exp2f((sh.target_at[a] - pm) * per_bit) / of_p.y;
                 float ux = sh.random[a];
                 if (draft) ux *= qm == -INFINITY ? 0.f : exp2f((sh.draft_at[a] - qm) * per_bit) / of_q.y;
-                fits = ux < px * (1.f - kNear);
-                unsure = !fits && !(ux > px * (1.f + kNear));
+                const bool few_bits = fmaxf(px, ux) < kFewBits;
+                fits = !few_bits && ux < px * (1.f - kNear);
+                unsure = few_bits || (!fits && !(ux > px * (1.f + kNear)));
             }
             if (fits) {
                 g++;
