@@ -195,6 +195,7 @@ def prepare(case: dict, seed: int) -> dict:
         s["buffers"] = _Buffers()
         made = {name: s["buffers"].of(x) for name, x in t.items()}
         s["h"], s["t"] = {name: m[0] for name, m in made.items()}, {name: m[1] for name, m in made.items()}
+        torch.cuda.synchronize()  # (they were copied on torch's stream, behind which the package's is not ordered)
     return s
 
 
@@ -264,6 +265,7 @@ def _plain_verify(case: dict, t: dict) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def run(state: dict):
+    """One pass.  With ``own`` it is under way on the package's stream: ``_backend.synchronize()``, or torch's of the device, before torch reads the outputs."""
     case, t = state["case"], state["t"]
     kind = case["kind"]
     if not own:
