@@ -286,7 +286,7 @@ int32_t yule_cuda_adapter_matmul_batched(yule_cuda_ctx *ctx, yule_buffer down, y
  * draft_stride apart, or handle 0 for drafts that were not drawn from a distribution (looked up, say); drafts: [n_seqs][n_draft] words; draft_lens: n_seqs
  * words, how many of them there are (handle 0: n_draft each; more count as n_draft); random: [n_seqs][n_draft + 1] floats in [0, 1).  With p, q the soft-max of
  * logits / temperature, draft t is accepted while random[t] * q(draft) < p(draft) (q = 1 without draft logits); at the first that is not, the token is
- * drawn from max(0, p - q), after the last accepted one from p: in index order, the first whose running sum exceeds random[n_draft] times the
+ * drawn from max(0, p - q) (from p if that is nothing), after the last accepted one from p: in index order, the first whose running sum exceeds random[n_draft] times the
  * whole.  Sums and exponentials are in 64 bits.  greedy != 0: drafts are accepted while they are the target's largest logit (ties to the highest
  * index, sampler.rs:150-163), the token is that logit's; draft_logits, random and temperature are then not looked at.
  * out_tokens: [n_seqs][n_draft + 1] words, the accepted drafts, the token after them, then 0xFFFFFFFF; out_accepted: n_seqs words, the number of accepted

@@ -215,6 +215,56 @@ def test_models_that_are_as_good_as_the_same(backend, V, step):
     c.check(backend)
 
 
+@pytest.mark.parametrize("V", [40, 300, 40000])
+@pytest.mark.parametrize("log_w", [-30, -37, -46, -120, -600])
+def test_what_p_has_more_of_is_next_to_nothing(backend, V, log_w):
+    """Both distributions are one token up to e^log_w, and the draft is neither's.  p has less of that token, by what it has more of the others in all, so w is p − q at the others,
+    of the size of e^log_w, where the whole of p is 1 or a few steps of 2^-52 from it."""
+    B = 24
+    c = Call(B=B, K=1, V=V, temperature=1.0)
+    r = np.random.default_rng(V - log_w)
+    others = 1 + r.permutation(V - 2)[:9]  # not the first token, nor the last, which is the draft
+    c.target[:], c.draft[:], c.drafts[:] = -np.inf, -np.inf, V - 1
+    c.target[:, :, 0], c.draft[:, :, 0] = 3.0, 3.0
+    c.target[:, :, others] = 3 + log_w + r.random((B, 2, 9))
+    c.draft[:, :, others] = np.nextafter(c.target[:, :1, others], np.float32(0)) - r.random((B, 1, 9)).astype(np.float32)
+    p, q = (np.exp(a[:, 0].astype(np.float64) - 3) for a in (c.target, c.draft))
+    # the wholes are 1 + sp and 1 + sq: their ratio from the difference of sp and sq
+    sp, sq = p[:, 1:].sum(-1, keepdims=True), q[:, 1:].sum(-1, keepdims=True)
+    w = np.maximum(p - q * ((sp - sq) / (1 + sq) + 1), 0)
+    w[:, 0] = 0
+    run = np.cumsum(w, -1)
+    for _ in range(100):
+        goal = c.random[:, 1].astype(np.float64)[:, None] * run[:, -1:]
+        near = (np.abs(run[:, others] - goal) / run[:, -1:]).min(-1) < 2.0 ** -10
+        if not near.any():
+            break
+        c.random[near, 1] = r.random(near.sum())
+    assert not near.any()
+    c.upload(backend).run(backend)
+    tokens, accepted = c.got(backend)
+    assert (accepted == 0).all() and (tokens[:, 0] == ((run > goal) & (w > 0)).argmax(-1)).all()
+
+
+def test_a_draft_that_the_same_distribution_does_not_have(backend):
+    """p = q: nothing is left of p − q, and the token is drawn from p."""
+    for V in (300, 40000):
+        c = Call(B=24, K=2, V=V, near=0.0)
+        c.drafts[:8, 0] = NONE
+        c.target[8:16, 0, 7] = c.draft[8:16, 0, 7] = -np.inf
+        c.drafts[8:16, 0] = 7
+        c.target[16:, 0, 5:] = c.draft[16:, 0, 5:] = -np.inf
+        c.drafts[16:, 0] = 9
+        c.upload(backend).run(backend)
+        tokens, accepted = c.got(backend)
+        assert (accepted == 0).all()
+        for b in range(24):
+            run = np.cumsum(soft(c.target[b, 0], c.temperature))
+            goal = float(c.random[b, 2]) * run[-1]
+            assert np.abs(run - goal).min() > 2.0 ** -29
+            assert tokens[b].tolist() == [np.nonzero(run > goal)[0][0], NONE, NONE]
+
+
 def test_random_numbers_at_the_ends(backend):
     for u in (0.0, np.nextafter(np.float32(1), np.float32(0))):
         c = Call(B=8, K=3, V=300)

@@ -16,8 +16,8 @@
 //
 // w takes one pass over its two rows, although it needs the sums of both first: with the ratio of the sums known to 2^-16, tokens with p > q are told from the others,
 // and Σ w over them is Σ exp_p − ratio · Σ exp_q with the ratio known by then.  A token on the wrong side has |p − q| below 2^-16 of p, so with the mass of all
-// tokens that near at most 2^-14 of Σ w, w is good to 2^-30; with more (models that are as good as the same) a second pass knows the ratio.  The share of the
-// vocabulary that holds the pick is gone through again with w itself.
+// tokens that near at most 2^-14 of Σ w, w is good to 2^-30; with more (models that are as good as the same) a second pass knows the ratio and adds w itself up,
+// which a difference of sums near 1 would lose below 2^-53.  Where w is nothing at all the token comes from p.  The share of the vocabulary that holds the pick is gone through again with w itself.
 
 #include <cfloat>
 #include <utility>
@@ -195,7 +195,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
     const uint32_t first = (warp % per_row) * 32 + lane, step = per_row * 32;  // (of fours of logits, or of single ones)
     uint32_t a = 0, g = p.group;  // the place in question, and which of its group it is
     uint32_t t0 = 0u - p.group, parity = 0, pass = 0;
-    double z[5], ratio;
+    double z[5], ratio, less;  // Σ w = z[2] − less · z[3]
+    bool alone = false;        // the token comes from p
     float pm, qm;
     const float *pr, *qr;
     uint32_t *out = p.tokens + (size_t)b * (p.n_draft + 1);
@@ -326,10 +327,11 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
             return;
         }
         // Not accepted, or too near to say, or the token behind the last draft: sums in 64 bits.
-        pr = target + (size_t)a * p.target_stride, qr = draft && a < k && qm != -INFINITY ? draft + (size_t)a * p.draft_stride : nullptr;
+        pr = target + (size_t)a * p.target_stride, qr = draft && a < k && qm != -INFINITY && !alone ? draft + (size_t)a * p.draft_stride : nullptr;
         const uint32_t without = !draft && a < k ? sh.drafts[a] : kNothing;
         ratio = qr ? (double)of_p.y / (double)of_q.y : 0.0;
-        for (bool known = !qr;;) {
+        bool known = !qr;
+        for (;;) {
             const Weight wp(pm, p.per_bit), wq(qr ? qm : 0.f, p.per_bit);
             double s0 = 0.0, s1 = 0.0, a0 = 0.0, a1 = 0.0, near = 0.0;
             const uint32_t i1 = min(lo + (warp + 1) * share, hi);
@@ -350,13 +352,13 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
                 load(i0 + kAhead * 32);
 #pragma unroll
                 for (int j = 0; j < kAhead; j++) {
-                const double e = wp(xs[j]);
+                    const double e = wp(xs[j]);
                     s0 += e;
                     if (qr) {
                         const double f = wq(ys[j]), d = fma(-ratio, f, e);
                         s1 += f;
                         const int of_d = __double2hiint(d);
-                        if (of_d >= 0) a0 += e, a1 += f;  // (a difference of zero adds nothing)
+                        if (of_d >= 0) a0 += known ? d : e, a1 += f;  // (a difference of zero adds nothing)
                         if ((of_d & 0x7FF00000) <= (__double2hiint(e) & 0x7FF00000) - (15 << 20)) near += e;  // |d| < 2^-14 e, and all below 2^-16
                     } else if (i0 + j * 32 != without) {
                         a0 += e;
@@ -384,27 +386,29 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
             if (known || !(z[4] > 0x1p-14 * (z[2] - ratio * z[3]))) break;
             known = true;
         }
-        if (unsure) {
+        if (unsure && !alone) {
             const double px = Weight(pm, p.per_bit)(sh.target_at[a]) / z[0], qx = !draft ? 1.0 : qr ? Weight(qm, p.per_bit)(sh.draft_at[a]) / z[1] : 0.0;
             if ((double)sh.random[a] * qx < px) {
                 g++;
                 continue;
             }
         }
-        break;
+        less = known ? 0.0 : ratio;
+        if (!qr || z[2] - less * z[3] > 0.0) break;
+        alone = true;  // nothing of w: p and q are the same, and a draft cannot be in either
     }
 
     // The token: the slice of the vocabulary in which the running sum passes the goal, and in it the warp's share (every warp for itself).
     const uint32_t without = !draft && a < k ? sh.drafts[a] : kNothing;
-    const double goal = (double)sh.last_random * (z[2] - ratio * z[3]);
+    const double goal = (double)sh.last_random * (z[2] - less * z[3]);
     double run = 0.0;
-    const uint32_t owner = part_of(lane < CTAS ? sh.exact[pass & 1u][2][lane] - ratio * sh.exact[pass & 1u][3][lane] : 0.0, goal, run);
+    const uint32_t owner = part_of(lane < CTAS ? sh.exact[pass & 1u][2][lane] - less * sh.exact[pass & 1u][3][lane] : 0.0, goal, run);
     if (owner == 16) {
         if (rank == 0) finish(kNothing);
         return;
     }
     if (rank != owner) return;
-    const uint32_t of_warp = part_of(lane < kWarps ? sh.warp_exact[2][lane] - ratio * sh.warp_exact[3][lane] : 0.0, goal, run) & 15u;
+    const uint32_t of_warp = part_of(lane < kWarps ? sh.warp_exact[2][lane] - less * sh.warp_exact[3][lane] : 0.0, goal, run) & 15u;
     // That share again, some consecutive tokens a thread: the first whose running sum passes the goal, else the last that is possible.
     const Weight wp(pm, p.per_bit), wq(qr ? qm : 0.f, p.per_bit);
     auto w_of = [&](uint32_t i) {
