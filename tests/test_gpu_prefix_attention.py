@@ -239,6 +239,23 @@ def test_sizes(backend, k, v):
     c.check(backend)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_dimensions_of_very_different_sizes(backend, hd, route):
+    """Per dimension of V: its error goes by the dimension's own largest |v|, and on the tensor core, where the numbers of 64 positions of V share a scale that leaves their largest at 2^13 or
+    more beside terms of fp16's 2^-24, by half a step of that: 2^-38 of the largest of all."""
+    c = Call(B=20, H=8, kv=2, hd=hd, P=300, C=30)
+    size = (2.0 ** -np.arange(hd)[::-1].clip(0, 26)).astype(np.float32)
+    c.pv *= size
+    c.tv *= size
+    out, _ = reference(c.q, c.pk, c.pv, c.tk, c.tv, c.lens)
+    _, of_one = reference(c.q, c.pk, np.ones_like(c.pv), c.tk, np.ones_like(c.tv), c.lens)  # tolerance where the largest is 1
+    largest = np.maximum(np.abs(c.pv).max((0, 1)), np.abs(c.tv).max((0, 1, 2))).astype(np.float64)  # of a dimension
+    tol = of_one[..., None] * largest + (0 if route in ("parts", "single") else 2.0 ** -38 * largest.max())
+    c.upload(backend).run(backend)
+    assert (np.abs(c.got(backend) - out) <= tol).all()
+    c.free(backend)
+
+
 def test_lengths_beyond_the_capacity(backend):
     a = Call(B=2, P=20, C=30, lens=[30, 30]).upload(backend)
     c = Call(B=2, P=20, C=30, lens=[31, 0xFFFFFFFF]).upload(backend)
@@ -268,6 +285,28 @@ def test_captured_and_replayed_with_other_lengths(backend):
         backend.graph_launch(g)
         c.check(backend)
     backend.graph_destroy(g)
+
+
+def test_graphs_captured_before_and_after_the_scratch_grew(route):
+    """One replays in the scratch that it was captured with, the other in the larger one, eager calls between them."""
+    b = CudaB200Backend(0)
+    small, large = Call(B=3, T=2, P=100, C=80).upload(b), Call(B=33, T=2, P=600, C=200).upload(b)
+    graphs = []
+    for c in (small, large):
+        c.run(b)
+        b.graph_begin()
+        c.run(b)
+        graphs.append(b.graph_end())
+    for first, second in ((0, 1), (1, 0)):
+        for c in (small, large):
+            b.copy_to_device(np.full(c.out_floats, 7.0, np.float32), c.h["out"])
+        b.graph_launch(graphs[first])
+        b.graph_launch(graphs[second])
+        small.check(b), large.check(b)
+        small.run(b), large.run(b)
+    for g in graphs:
+        b.graph_destroy(g)
+    b.close()
 
 
 def test_a_capture_cannot_grow_the_scratch(route):

@@ -75,3 +75,32 @@ def test_samples(backend):
     assert together(jobs) == want
     for h in logits:
         backend.free(h)
+
+
+def test_operators_of_a_served_batch(backend):
+    """Attention behind a prefix (all its routes by size), adapters and verification of several threads share the context's scratch, which grows meanwhile."""
+    from test_gpu_adapters import Call as Adapters
+    from test_gpu_prefix_attention import Call as Attention
+    from test_gpu_verify_drafts import Call as Verify
+    from yule_b200 import CudaB200Backend
+    calls = [Attention(B=2, P=40, C=30, H=8, kv=2, hd=64), Attention(B=9, T=3, P=700, C=90, H=8, kv=2, hd=96), Attention(B=16, T=2, P=2000, C=60, H=32, kv=8, hd=128),
+             Adapters(batch=20), Adapters(batch=400, rows=300, cols=512), Adapters(batch=300, rank=100, dtype=DType.F32), Verify(V=9000), Verify(B=20, V=3000, by="lookup", greedy=True)]
+
+    def job(c, b):
+        got = []
+        for _ in range(25):
+            c.run(b)
+            got += list(c.got(b)) if isinstance(c, Verify) else [c.got(b)]
+        return got
+    want = []
+    for c in calls:
+        c.upload(backend)
+        want.append(job(c, backend))
+        c.check(backend)
+        c.free(backend)
+    for _ in range(2):
+        b = CudaB200Backend(0)  # without scratch yet
+        for c in calls:
+            c.upload(b)
+        assert all(same(g, w) for g, w in zip(together([lambda c=c: job(c, b) for c in calls]), want))
+        b.close()
