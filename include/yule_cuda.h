@@ -244,8 +244,8 @@ int32_t yule_cuda_embed_gather(yule_cuda_ctx *ctx, yule_buffer table, uint32_t g
 
 /* ── a batch of sequences served together (no counterpart in the reference, which serves one sequence per ModelRunner,
  *    yule-infer/src/lib.rs:169-216) ──────────────────────────────────────────
- * Lengths, adapters and drafts are read on the device, so a captured call can be replayed with others.  The calls share a scratch
- * that the context grows on demand; growing is not possible while a graph is being captured, so run one call of the
+ * Lengths, adapters and drafts are read on the device, so a captured call can be replayed with others.  Attention, and adapters of
+ * more than 128 rows, share a scratch that the context grows on demand; growing is not possible while a graph is being captured, so run one call of the
  * same sizes before yule_cuda_graph_begin. */
 
 /* Decode attention of n_seqs sequences that share a prefix, n_query query tokens each (1, or 1 + drafted tokens).  Keys of every row: positions
@@ -254,8 +254,10 @@ int32_t yule_cuda_embed_gather(yule_cuda_ctx *ctx, yule_buffer table, uint32_t g
  * tail_stride apart.  tail_lens: n_seqs words, the positions that sequence b's own caches hold, its query tokens' among them (the newest n_query; more than
  * tail_capacity counts as tail_capacity): query token t sees its own and earlier ones, tail_lens[b] - (n_query - 1 - t) positions, none if that is negative.
  * A row that sees nothing is zero.  Scores, soft-max and head grouping as yule_cuda_multihead_attention.  Handles of a prefix_len
- * or tail_capacity of 0 are not looked at.  A value that is not finite in a position that a row sees makes that row's output not finite; what a
- * row does not see does not count for it, whatever it holds.  head_dim a multiple of 4, at most 256; strides multiples of 4; n_query at most 64, n_kv_heads
+ * or tail_capacity of 0 are not looked at.  What is not finite in K, in a position that a row sees, leaves no number of that row's output
+ * finite, in V not the one of its dimension (nor, perhaps, others); what a row does not see does not count for it, whatever it holds.  Products are those of 32 bits up to 2^-20 of their size, with
+ * one exception: behind a prefix that 32 rows or more share (head_dim 64 or 128, as many positions as make the tensor core pay), the numbers of a query row, and of K or V in 64 positions of
+ * a KV head, are kept with an error of 2^-38 of the largest of them at the least, so that those below 2^-14 of it have fewer bits than 22.  head_dim a multiple of 4, at most 256; strides multiples of 4; n_query at most 64, n_kv_heads
  * at most 65535, prefix_len and n_seqs * tail_capacity at most 2^31 - 1. */
 typedef struct yule_prefix_attention {
     uint32_t head_dim, n_heads, n_kv_heads;
@@ -287,10 +289,11 @@ int32_t yule_cuda_adapter_matmul_batched(yule_cuda_ctx *ctx, yule_buffer down, y
  * words, how many of them there are (handle 0: n_draft each; more count as n_draft); random: [n_seqs][n_draft + 1] floats in [0, 1).  With p, q the soft-max of
  * logits / temperature, draft t is accepted while random[t] * q(draft) < p(draft) (q = 1 without draft logits); at the first that is not, the token is
  * drawn from max(0, p - q) (from p if that is nothing), after the last accepted one from p: in index order, the first whose running sum exceeds random[n_draft] times the
- * whole.  Sums and exponentials are in 64 bits.  greedy != 0: drafts are accepted while they are the target's largest logit (ties to the highest
+ * whole.  The token is drawn with sums in 64 bits, of exponentials good to 2^-34; acceptances are decided in 32 bits, and
+ * again in 64 where the sides are within 2^-13 of one another or both below 2^-100.  greedy != 0: drafts are accepted while they are the target's largest logit (ties to the highest
  * index, sampler.rs:150-163), the token is that logit's; draft_logits, random and temperature are then not looked at.
  * out_tokens: [n_seqs][n_draft + 1] words, the accepted drafts, the token after them, then 0xFFFFFFFF; out_accepted: n_seqs words, the number of accepted
- * drafts.  A logit that is NaN or -infinity is a token that cannot be; a row of those accepts nothing and gives 0xFFFFFFFF; a draft outside the
+ * drafts.  A logit that is NaN or -infinity is a token that cannot be; a target row of those accepts nothing and gives 0xFFFFFFFF, in a draft row of those q is 0; a draft outside the
  * vocabulary is not accepted.  Penalties and cut-offs of yule_cuda_sample are not applied.  vocab_size at most 2^24, n_seqs 65536, n_draft from 1 to 256,
  * temperature from 1e-6 to 1e6. */
 typedef struct yule_verification {

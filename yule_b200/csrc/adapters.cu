@@ -9,7 +9,7 @@
 // Decode steps (tiles of 8): one launch, a cluster of CTAs per slot.  What there is to read is an adapter's 0.1 to 2 MB, so time goes by in latency: a CTA takes
 // a share of the columns for all ranks, writes its sums into every other CTA's shared memory, and has its share of the outputs, whose first rows of `up` and of
 // base it loads before the barrier.  32 requests of as many adapters of rank 16 beside 4096 × 4096: 7.4 us a call (two launches, with the sums through the scratch:
-// 12.2; 8.4 MB at the rate of a copy: 1.3), one token beside 2048 × 2048: 5.5 (7.5), of which the call itself is the most.
+// 12.2; 8.4 MB at the rate of a copy: 1.3), one token beside 2048 × 2048: 5.8 (7.5), of which the call itself is the most.
 //
 // Prompts (tiles of 32): two launches, since base and output are most of the traffic and want CTAs of their own.  1501 rows of six requests, rank 64, beside 14336 × 4096:
 // 71 us, the first launch 22 of them, the second 51 for 195 MB; both are bound by the instructions around the copies and products, not by memory

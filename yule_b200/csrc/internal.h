@@ -27,7 +27,7 @@ namespace yule {
 
 // Values of the device status word (yule_cuda_ctx::device_status): which bounded wait gave up.
 constexpr int kStatusPeerTimeout = 2;   // tensor parallelism: a peer's (value, epoch) pairs or flag never arrived
-constexpr int kStatusGemmTimeout = 3;   // tcgen05 GEMM: an mbarrier of its pipeline never completed
+constexpr int kStatusPipelineTimeout = 3;  // tcgen05 GEMM, attention of prompts or behind a shared prefix: an mbarrier of a pipeline never completed
 constexpr int kStatusRingTimeout = 4;   // matvec: a bulk copy into the shared-memory ring never completed
 // Default budget of a bounded wait, in SM clock cycles (~1 s): far beyond any real skew between ranks,
 // short enough to report a lost peer.  yule_cuda_set_wait_budget changes it per context.
@@ -44,7 +44,7 @@ struct Buffer {
     uint32_t planar_cols = 0;  // the copy is laid out row by row, so it belongs to one (rows, cols) shape
 };
 
-// Tuning and timing knobs (YULE_QMV_*, YULE_GEMM_*, YULE_CUDA_*, YULE_TP_*) are read from the environment only
+// Tuning and timing knobs (YULE_QMV_*, YULE_GEMM_*, YULE_CUDA_*, YULE_TP_*, YULE_PREFIX_*) are read from the environment only
 // when the process runs with YULE_CUDA_DEBUG=1; a production process ignores them, so no environment
 // variable can change routing or results.  Returns the variable's value or null.
 const char *knob(const char *name);
@@ -94,7 +94,7 @@ struct yule_cuda_ctx {
     // scratch of the device sampler (sampler.cu): probabilities and occurrence counts, plus one word for the pick
     float *sampler_scratch = nullptr;
     size_t sampler_scratch_floats = 0;
-    // scratch of the operators for a batch served together (prefix_attention.cu, adapters.cu, verify.cu), grown on demand: each call's first kernel waits for
+    // scratch of the operators for a batch served together (prefix_attention.cu, adapters.cu), grown on demand: each call's first kernel waits for
     // all before it, so they can share it
     void *batch_scratch = nullptr;
     size_t batch_scratch_bytes = 0;

@@ -153,8 +153,8 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
     };
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
     for (uint32_t tile = warp; tile < n_tiles; tile += kWarps, phase ^= 1u) {
-        const uint32_t n = SINGLE && tile < of_it ? p.prefix_len - tile * kKeys : key1 - key0 - (tile - of_it) * kKeys;  // positions from the tile's first on (what lies behind, in the tile or the row, may be anything)
-        const bool whole = n >= (uint32_t)kKeys, in0 = turned < n, in1 = turned + 8 < n;
+        const uint32_t there = SINGLE && tile < of_it ? p.prefix_len - tile * kKeys : key1 - key0 - (tile - of_it) * kKeys;  // positions from the tile's first on (what lies behind, in the tile or the row, may be anything)
+        const bool whole = there >= (uint32_t)kKeys, in0 = turned < there, in1 = turned + 8 < there;
         // Scores of positions base + turned and base + turned + 8.  The tensor core truncates what it adds to, so the large products of four steps at a time have sums of their own.
         // (With few query rows a sum of all small products would be a chain of as many steps as there are products: four sums.)
         constexpr int kSums = ROWS == 1 ? 4 : 1;
@@ -250,8 +250,8 @@ __global__ void __launch_bounds__(kWarps * 32) prefix_part_kernel(const __grid_c
                 float4 a = *reinterpret_cast<const float4 *>(at + ((turned ^ t) << 4)), b = *reinterpret_cast<const float4 *>(at + 4 * 128 + ((turned ^ (t + 4)) << 4));
                 if (!EXACT && 32 * i + 4 * turned >= p.hd) a = b = zero;
                 if (!whole) {
-                    if (8 * u + t >= n) a = zero;
-                    if (8 * u + t + 4 >= n) b = zero;
+                    if (8 * u + t >= there) a = zero;
+                    if (8 * u + t + 4 >= there) b = zero;
                 }
                 uint32_t ah[4], al[4], bh[4], bl[4];
                 split_tf32(a.x, ah[0], al[0]), split_tf32(a.y, ah[1], al[1]), split_tf32(a.z, ah[2], al[2]), split_tf32(a.w, ah[3], al[3]);

@@ -79,7 +79,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
             if (*abort_flag) return false;
             if (clock64() - t0 > kWaitCycles) {
                 *abort_flag = 1;
-                atomicExch(status, kStatusGemmTimeout);
+                atomicExch(status, kStatusPipelineTimeout);
                 return false;
             }
         }
